@@ -304,6 +304,91 @@ int wkvm_gdn_prefill_slots(
     int32_t* status, wkvm_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * Selective state space layers: a short causal convolution and a selective
+ * scan, each with its per-request state in a bank slot, for prompts and for
+ * single tokens. No wkvm caller exists (wkvm runs RWKV-7 only); the short
+ * convolution also stands before q, k and v in gated-delta-rule layers.
+ *
+ * Sequences are a batch [B, T, ..] (cu_seqlens NULL) or B sequences packed
+ * along one token axis of T tokens in all (cu_seqlens: int64 device [B+1]).
+ * A sequence may be empty: its state stays as it is. Tokens of a packed
+ * axis that no sequence covers are neither read nor written. Offsets that
+ * descend or leave the axis are reported as WKVM_ERR_INVALID_ARG in
+ * `status` and their sequence is skipped. Inputs may be strided over batch
+ * and tokens (strides in elements; channels are contiguous); outputs are
+ * contiguous and must not overlap an input.
+ * ------------------------------------------------------------------------ */
+
+enum { WKVM_ACT_NONE = 0, WKVM_ACT_SILU = 1 };
+
+/* Short causal convolution of width W (2, 3 or 4) over channels:
+ *   o[t][d] = act(bias[d] + sum_j weight[d][j] x[t - W + 1 + j][d])
+ * weight [D, W], bias [D] or NULL, in the activations' dtype. The inputs
+ * before a sequence's first token come from its state row [W-1, D], oldest
+ * first, same dtype (s0 NULL: zeros), and the row then holds the last W-1
+ * inputs (`st`, optional; s0 == st is allowed). Sums are fp32. */
+int wkvm_short_conv(
+    const void* x, int64_t x_batch_stride, int64_t x_token_stride, const void* weight,
+    const void* bias, void* o, const void* s0, void* st, const int64_t* cu_seqlens,
+    int32_t B, int32_t T, int32_t D, int32_t W, int32_t activation, int32_t dtype,
+    int32_t* status, wkvm_stream_t stream);
+
+/* The same with the state rows of sequence i in bank_layer[slot_ids[i]]
+ * ([num_slots, W-1, D]), read and written in place. */
+int wkvm_short_conv_slots(
+    const void* x, int64_t x_batch_stride, int64_t x_token_stride, const void* weight,
+    const void* bias, void* o, void* bank_layer, int64_t num_slots, const int32_t* slot_ids,
+    const int64_t* cu_seqlens, int32_t B, int32_t T, int32_t D, int32_t W,
+    int32_t activation, int32_t dtype, int32_t* status, wkvm_stream_t stream);
+
+/* Selective scan. Per token, channel d (of D) and state n (of N):
+ *   delta = dt[d] + dt_bias[d], through log(1 + e^x) when softplus != 0
+ *   h[d][n] = exp(delta A[d][n]) h[d][n] + delta x[d] B[g][n]
+ *   o[d] = (sum_n C[g][n] h[d][n] + D_skip[d] x[d]) silu(z[d])
+ * x, dt, z (or NULL) are [.., D] and Bm, Cm [.., G, N] rows in `dtype`,
+ * g = d / (D / G), N in {8, 16, 32, 64, 128}; A [D, N], D_skip [D] or NULL
+ * and dt_bias [D] or NULL are fp32; states are fp32 [.., D, N]. `strides`
+ * is a host array of ten: batch and token stride of x, dt, z, Bm, Cm.
+ * h0 (optional) and ht (optional, may equal h0) are [B, D, N]. */
+int wkvm_selective_scan(
+    const void* x, const void* dt, const float* A, const void* Bm, const void* Cm,
+    const float* D_skip, const void* z, const float* dt_bias, void* o,
+    const int64_t* strides, const float* h0, float* ht, const int64_t* cu_seqlens,
+    int32_t B, int32_t T, int32_t D, int32_t N, int32_t G, int32_t softplus,
+    int32_t dtype, int32_t* status, wkvm_stream_t stream);
+
+/* The same with the state of sequence i in bank_layer[slot_ids[i]]
+ * ([num_slots, D, N] fp32), read and written in place. */
+int wkvm_selective_scan_slots(
+    const void* x, const void* dt, const float* A, const void* Bm, const void* Cm,
+    const float* D_skip, const void* z, const float* dt_bias, void* o,
+    const int64_t* strides, float* bank_layer, int64_t num_slots,
+    const int32_t* slot_ids, const int64_t* cu_seqlens, int32_t B, int32_t T,
+    int32_t D, int32_t N, int32_t G, int32_t softplus, int32_t dtype,
+    int32_t* status, wkvm_stream_t stream);
+
+/* Chooses one token for each of B rows of V logits (row_stride elements
+ * apart) from a given uniform number u[b] in [0, 1). With m the row's
+ * largest logit and w_i = exp((l_i - m) / temperature):
+ *   top_k  keeps the k largest logits (k <= 0: all);
+ *   top_p  keeps, of those in descending order, the shortest prefix whose
+ *          mass is >= top_p of theirs, at least one (>= 1: all);
+ *   min_p  keeps, of those, w_i >= min_p (<= 0: all; the largest is kept);
+ *   token  = the first kept id whose running mass over ascending ids is
+ *            > u times the mass kept; logprob = log(w_token / mass kept).
+ * Ties go to the lowest ids. temperature <= 0 is greedy: the largest logit,
+ * logprob 0. -inf and NaN logits are never chosen, +inf ones share the whole
+ * mass, and a row with nothing to choose gives token -1 and logprob -inf.
+ * Masses are fp64-accurate and summed in a fixed order: the same inputs give
+ * the same token on every run. Each setting is a device array [B], or NULL
+ * and the scalar beside it holds for every row. */
+int wkvm_sample_tokens(
+    const void* logits, int64_t row_stride, const float* u, const float* temperature,
+    const int32_t* top_k, const float* top_p, const float* min_p, float temperature0,
+    int32_t top_k0, float top_p0, float min_p0, int64_t* tokens, float* logprobs,
+    int32_t B, int32_t V, int32_t dtype, wkvm_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * Slot copies. A state family tensor is viewed as [outer, num_slots, row]:
  * bank.wkv [L, S+1, H*K*V fp32] has outer = L; bank.shift [L, 2, S+1, D]
  * has outer = 2L. `outer_stride` and `slot_stride` are in bytes, `row_bytes`

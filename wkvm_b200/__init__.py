@@ -18,6 +18,15 @@ from .ops import (
     wkv7_decode_slots,
     wkv7_prefill_slots,
 )
+from .sampling import sample_tokens
+from .ssm import (
+    selective_scan,
+    selective_scan_decode_slots,
+    selective_scan_prefill_slots,
+    short_conv,
+    short_conv_decode_slots,
+    short_conv_prefill_slots,
+)
 
 __all__ = [
     "ops",
@@ -28,6 +37,13 @@ __all__ = [
     "fused_recurrent_rwkv7",
     "gdn_decode_slots",
     "gdn_prefill_slots",
+    "sample_tokens",
+    "selective_scan",
+    "selective_scan_decode_slots",
+    "selective_scan_prefill_slots",
+    "short_conv",
+    "short_conv_decode_slots",
+    "short_conv_prefill_slots",
     "wkv7_decode_slots",
     "wkv7_prefill_slots",
 ]

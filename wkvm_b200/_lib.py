@@ -47,6 +47,11 @@ SIGNATURES: dict[str, list] = {
     "wkvm_gdn_chunk_workspace_bytes": [I32] * 5,
     "wkvm_wkv7_shift_mix_slots": [P, P, P, I64, I64, P, P, I32, I32, I32, I32, P, P],
     "wkvm_chunk_gated_delta_rule_static": [P] * 6 + [P, P, P] + [I32] * 6 + [F32, I32, I32, P, P],
+    "wkvm_short_conv": [P, I64, I64, P, P, P, P, P, P] + [I32] * 6 + [P, P],
+    "wkvm_short_conv_slots": [P, I64, I64, P, P, P, P, I64, P, P] + [I32] * 6 + [P, P],
+    "wkvm_selective_scan": [P] * 9 + [P, P, P, P] + [I32] * 7 + [P, P],
+    "wkvm_selective_scan_slots": [P] * 9 + [P, P, I64, P, P] + [I32] * 7 + [P, P],
+    "wkvm_sample_tokens": [P, I64] + [P] * 5 + [F32, I32, F32, F32] + [P, P, I32, I32, I32, P],
 }
 
 RESTYPES = {

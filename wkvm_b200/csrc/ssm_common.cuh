@@ -1,0 +1,76 @@
+// What the short convolution and the selective scan share: where a sequence's
+// tokens and its state row lie, and 32-bit activation functions.
+#pragma once
+
+#include "common.cuh"
+
+namespace wkvm {
+
+// Sequences of one call: a batch [nseq, T] (cu null), or packed along one
+// token axis of T tokens in all (cu: nseq + 1 ascending offsets).
+struct Seqs {
+  const int64_t* cu;
+  int32_t nseq;
+  int32_t T;
+};
+
+struct SeqSpan {
+  int64_t bos, len;  // first token on the flattened token axis, token count
+  bool ok;           // false: offsets that leave the token axis or descend
+};
+
+__device__ __forceinline__ SeqSpan seq_span(const Seqs& s, int n) {
+  if (!s.cu) return {(int64_t)n * s.T, s.T, true};
+  const int64_t b = s.cu[n], e = s.cu[n + 1];
+  const bool ok = b >= 0 && e >= b && e <= s.T;
+  return {ok ? b : 0, ok ? e - b : 0, ok};
+}
+
+// An activation tensor: element (sequence n, its token t, channel c) at
+// p[n * bs + t * ts + c], or p[(bos + t) * ts + c] when packed.
+struct Act {
+  const void* p;
+  int64_t bs, ts;  // elements
+};
+
+__device__ __forceinline__ int64_t act_row(const Seqs& s, const Act& a, int n, int64_t bos) {
+  return s.cu ? bos * a.ts : n * a.bs;
+}
+
+// The row of the state tensor that sequence n reads and writes: its slot, or
+// n itself without slot ids. A slot id outside the bank is reported and its
+// sequence skipped.
+__device__ __forceinline__ bool state_row(const int32_t* ids, int64_t num_slots, int n,
+                                          int64_t* row) {
+  *row = ids ? (int64_t)ids[n] : n;
+  return !ids || (*row >= 0 && *row < num_slots);
+}
+
+// x * sigmoid(x). EXACT: the 32-bit functions (fp32 outputs); otherwise the
+// hardware approximations, whose 2^-21 is far below a 16-bit output's
+// rounding.
+template <bool EXACT>
+__device__ __forceinline__ float silu(float x) {
+  if constexpr (EXACT) return x / (1.0f + expf(-x));
+  return __fdividef(x, 1.0f + __expf(-x));
+}
+
+// log(1 + e^x) without losing small values: max(x, 0) + log1p(e^-|x|). The
+// result scales every exponent of the scan, so it is computed to fp32.
+__device__ __forceinline__ float softplus(float x) {
+  return fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x))) + (x != x ? x : 0.0f);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+inline bool aligned_to(const void* p, uintptr_t n) {
+  return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0;
+}
+
+}  // namespace wkvm
