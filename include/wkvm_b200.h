@@ -386,7 +386,7 @@ int wkvm_sample_tokens(
     const void* logits, int64_t row_stride, const float* u, const float* temperature,
     const int32_t* top_k, const float* top_p, const float* min_p, float temperature0,
     int32_t top_k0, float top_p0, float min_p0, int64_t* tokens, float* logprobs,
-    int32_t B, int32_t V, int32_t dtype, wkvm_stream_t stream);
+    int32_t B, int32_t V, int32_t dtype, int32_t* status, wkvm_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * Slot copies. A state family tensor is viewed as [outer, num_slots, row]:

@@ -128,15 +128,13 @@ def test_sampling_refusals(anywhere):
 
 def test_strides_given_to_the_kernels():
     t = torch.zeros(4, 5, 6)
-    assert ssm._rows(t)[1:] == (30, 6)
+    assert ssm._rows(t)[0] is t and ssm._rows(t)[1] == (30, 6, 1)
     half = torch.zeros(4, 5, 12)[..., 6:]
-    assert ssm._rows(half)[0] is half and ssm._rows(half)[1:] == (60, 12)
-    one = torch.zeros(1, 1, 12)[..., 1:7]
-    assert ssm._rows(one)[1:] == (0, 0)
+    assert ssm._rows(half)[0] is half and ssm._rows(half)[1] == (60, 12, 1)
     turned = torch.zeros(4, 6, 5).transpose(1, 2)
-    assert ssm._rows(turned)[0].is_contiguous() and ssm._rows(turned)[1:] == (30, 6)
+    assert ssm._rows(turned)[0].is_contiguous() and ssm._rows(turned)[1] == (30, 6, 1)
     groups = torch.zeros(4, 5, 40)[..., 3:35].unflatten(-1, (2, 16))
-    assert ssm._rows(groups, 2)[0] is groups and ssm._rows(groups, 2)[1:] == (200, 40)
+    assert ssm._rows(groups, 2)[0] is groups and ssm._rows(groups, 2)[1] == (200, 40, 16, 1)
     gapped = torch.zeros(4, 5, 2, 20)[..., :16]
     assert ssm._rows(gapped, 2)[0].is_contiguous()
 
@@ -170,7 +168,7 @@ def test_c_entry_refusals(lib):
 
     def sample(B=1, V=8, dt=1, x=d, u=d, o=d):
         f = ctypes.c_float
-        return lib.wkvm_sample_tokens(x, 8, u, n, n, n, n, f(1), 0, f(1), f(0), o, o, B, V, dt, n)
+        return lib.wkvm_sample_tokens(x, 8, u, n, n, n, n, f(1), 0, f(1), f(0), o, o, B, V, dt, n, n)
 
     assert sample(B=-1) == -1 and sample(V=0) == -1 and sample(dt=5) == -3 and sample(x=n) == -1
     assert sample(u=n) == -1 and sample(o=n) == -1 and sample(B=0) == 0

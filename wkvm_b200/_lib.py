@@ -51,7 +51,7 @@ SIGNATURES: dict[str, list] = {
     "wkvm_short_conv_slots": [P, I64, I64, P, P, P, P, I64, P, P] + [I32] * 6 + [P, P],
     "wkvm_selective_scan": [P] * 9 + [P, P, P, P] + [I32] * 7 + [P, P],
     "wkvm_selective_scan_slots": [P] * 9 + [P, P, I64, P, P] + [I32] * 7 + [P, P],
-    "wkvm_sample_tokens": [P, I64] + [P] * 5 + [F32, I32, F32, F32] + [P, P, I32, I32, I32, P],
+    "wkvm_sample_tokens": [P, I64] + [P] * 5 + [F32, I32, F32, F32] + [P, P, I32, I32, I32, P, P],
 }
 
 RESTYPES = {
@@ -112,9 +112,8 @@ post_call = None
 
 def call(name: str, *args) -> None:
     """Calls an entry point and raises WkvmError on a nonzero return."""
-    lib = load()
-    fn = getattr(lib, name)
-    rc = fn(*args)
+    lib = _lib if _lib is not None else load()
+    rc = getattr(lib, name)(*args)
     if rc != 0:
         raise WkvmError(name, rc)
     if post_call is not None:

@@ -31,6 +31,7 @@ struct SampleArgs {
   int64_t* token;
   float* logprob;
   int32_t B, V;
+  int* status;
 };
 
 // Ascending unsigned order of floats; NaN and -inf become 0 (never kept).
@@ -211,14 +212,14 @@ extern "C" int wkvm_sample_tokens(const void* logits, int64_t row_stride, const 
                                   const float* top_p, const float* min_p, float temperature0,
                                   int32_t top_k0, float top_p0, float min_p0, int64_t* tokens,
                                   float* logprobs, int32_t B, int32_t V, int32_t dtype,
-                                  wkvm_stream_t stream) {
+                                  int32_t* status, wkvm_stream_t stream) {
   if (B < 0 || V <= 0) return WKVM_ERR_INVALID_ARG;
   if (dtype != WKVM_DTYPE_F32 && dtype != WKVM_DTYPE_BF16 && dtype != WKVM_DTYPE_F16)
     return WKVM_ERR_DTYPE;
   if (B == 0) return WKVM_OK;
   if (!logits || !u || !tokens || !logprobs) return WKVM_ERR_INVALID_ARG;
   wkvm::SampleArgs a{logits, row_stride, u, temperature, top_p, min_p, top_k, temperature0,
-                     top_p0, min_p0, top_k0, tokens, logprobs, B, V};
+                     top_p0, min_p0, top_k0, tokens, logprobs, B, V, status};
   cudaStream_t st = (cudaStream_t)stream;
   switch (dtype) {
     case WKVM_DTYPE_F32: wkvm::sample_kernel<float><<<B, wkvm::kThreads, 0, st>>>(a); break;

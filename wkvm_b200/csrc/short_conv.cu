@@ -217,7 +217,8 @@ int launch_conv(const ConvArgs& a, int W, bool silu, cudaStream_t st) {
   return vec ? launch_conv_v<T, V>(a, W, silu, st) : launch_conv_v<T, 1>(a, W, silu, st);
 }
 
-int run_conv(const ConvArgs& a, int W, int act, int dtype, cudaStream_t st) {
+int run_conv(ConvArgs a, int W, int act, int dtype, cudaStream_t st) {
+  a.x = plain_strides(a.x, a.seqs);
   if (a.seqs.nseq < 0 || a.seqs.T < 0 || a.D <= 0) return WKVM_ERR_INVALID_ARG;
   if (act != WKVM_ACT_NONE && act != WKVM_ACT_SILU) return WKVM_ERR_INVALID_ARG;
   if (W < 2 || W > 4) return WKVM_ERR_SHAPE;

@@ -59,6 +59,20 @@ def status_word(device: torch.device | int | str | None = None) -> torch.Tensor:
     return t
 
 
+def _launch(name: str, idx: int, *args) -> None:
+    """Calls an entry point that ends in (status, stream) on device ``idx``,
+    on that device's current stream. Single-token calls are bound by the
+    host, so the device is switched only when it is not the current one."""
+    st = _status.get(idx)
+    if st is None:
+        st = status_word(idx)
+    if torch._C._cuda_getDevice() == idx:
+        _lib.call(name, *args, st.data_ptr(), torch._C._cuda_getCurrentRawStream(idx))
+    else:
+        with torch.cuda.device(idx):
+            _lib.call(name, *args, st.data_ptr(), torch._C._cuda_getCurrentRawStream(idx))
+
+
 def check_device_status(device=None, reset: bool = True) -> None:
     """Synchronises with the device's status word and raises the first
     recorded device-side error (e.g. an out-of-range slot id)."""

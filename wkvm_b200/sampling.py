@@ -8,15 +8,19 @@ from . import _lib
 from . import ops as _ops
 
 
-def _setting(name: str, value, rows: int, dtype: torch.dtype, device):
+def _setting(name: str, value, rows: int, dtype: torch.dtype, logits: torch.Tensor):
     """(per-row device tensor or None, scalar) of one sampling setting."""
     if not isinstance(value, torch.Tensor):
+        if value is None or not value >= 0:
+            raise ValueError(f"{name} must be >= 0, not {value!r}")
         return None, value
     if value.dim() == 0:
         value = value.expand(rows)
-    if tuple(value.shape) != (rows,):
+    if value.dim() != 1 or value.shape[0] != rows:
         raise ValueError(f"{name} must be a number or [{rows}], not {tuple(value.shape)}")
-    return value.to(device=device, dtype=dtype).contiguous(), 0
+    if value.dtype is dtype and value.get_device() == logits.get_device() and value.is_contiguous():
+        return value, 0
+    return value.to(device=logits.device, dtype=dtype).contiguous(), 0
 
 
 def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0,
@@ -35,7 +39,11 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     logits are never chosen; a row of nothing else gives token -1 and
     log-probability -inf. The same inputs give the same tokens on every run,
     eagerly and in a captured graph."""
-    _ops._require_cuda(logits, u)
+    idx = logits.get_device()
+    if idx < 0 or u.get_device() != idx:
+        _ops._require_cuda(logits, u)
+        if u.device != logits.device:
+            raise ValueError(f"u must be on {logits.device}, not {u.device}")
     if logits.dim() != 2:
         raise ValueError(f"logits must be [B, V], not {tuple(logits.shape)}")
     if logits.dtype not in _ops._DTYPES:
@@ -43,26 +51,24 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     B, V = logits.shape
     if V < 1 or V >= 1 << 31:
         raise ValueError(f"a vocabulary of {V} is not supported")
-    if tuple(u.shape) != (B,) or u.device != logits.device:
-        raise ValueError(f"u must be [{B}] on {logits.device}")
-    dev = logits.device
-    temp, temp0 = _setting("temperature", temperature, B, torch.float32, dev)
-    k, k0 = _setting("top_k", top_k, B, torch.int32, dev)
-    tp, tp0 = _setting("top_p", top_p, B, torch.float32, dev)
-    mp, mp0 = _setting("min_p", min_p, B, torch.float32, dev)
-    for name, v in (("temperature", temp0), ("top_k", k0), ("top_p", tp0), ("min_p", mp0)):
-        if v is None or not v >= 0:
-            raise ValueError(f"{name} must be >= 0, not {v!r}")
+    if u.dim() != 1 or u.shape[0] != B:
+        raise ValueError(f"u must be [{B}], not {tuple(u.shape)}")
+    temp, temp0 = _setting("temperature", temperature, B, torch.float32, logits)
+    k, k0 = _setting("top_k", top_k, B, torch.int32, logits)
+    tp, tp0 = _setting("top_p", top_p, B, torch.float32, logits)
+    mp, mp0 = _setting("min_p", min_p, B, torch.float32, logits)
     if mp0 > 1:
         raise ValueError(f"min_p must be <= 1, not {mp0!r}")
-    if V > 1 and logits.stride(1) != 1:
+    stride, last = logits.stride()
+    if last != 1 and V > 1:
         logits = logits.contiguous()
-    u = u.to(torch.float32).contiguous()
-    tokens = torch.empty(B, dtype=torch.int64, device=dev)
-    logprobs = torch.empty(B, dtype=torch.float32, device=dev)
+        stride = V
+    if u.dtype is not torch.float32 or not u.is_contiguous():
+        u = u.to(torch.float32).contiguous()
+    tokens = torch.empty(B, dtype=torch.int64, device=logits.device)
+    logprobs = torch.empty(B, dtype=torch.float32, device=logits.device)
     p = _ops._ptr
-    with torch.cuda.device(dev):
-        _lib.call("wkvm_sample_tokens", p(logits), logits.stride(0) if B > 1 else V, p(u), p(temp), p(k),
-                  p(tp), p(mp), float(temp0), min(int(k0), V), float(tp0), float(mp0), p(tokens), p(logprobs),
-                  B, V, _ops._DTYPES[logits.dtype], _ops._stream(dev))
+    _ops._launch("wkvm_sample_tokens", idx, logits.data_ptr(), stride, u.data_ptr(), p(temp), p(k), p(tp), p(mp),
+                 float(temp0), min(int(k0), V), float(tp0), float(mp0), tokens.data_ptr(), logprobs.data_ptr(), B, V,
+                 _ops._DTYPES[logits.dtype])
     return tokens, logprobs

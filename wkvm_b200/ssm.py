@@ -27,58 +27,64 @@ from . import ops as _ops
 _STATES = (8, 16, 32, 64, 128)
 _WIDTHS = (2, 3, 4)
 _ACTIVATIONS = {None: 0, "silu": 1, "swish": 1}
+_Strides = ctypes.c_int64 * 10
 
 
-def _no_grad(*ts):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        raise RuntimeError("this operator has no backward pass: call it under torch.no_grad() or "
-                           "with detached tensors")
-
-
-def _same_device(*ts):
-    _ops._require_cuda(*ts)
-    ts = [t for t in ts if t is not None]
-    if any(t.device != ts[0].device for t in ts):
-        raise ValueError(f"tensors lie on different devices: {sorted({str(t.device) for t in ts})}")
-
-
-def _rows(t: torch.Tensor | None, tail: int = 1):
-    """(tensor, batch stride, token stride): ``t`` itself when its last
-    ``tail`` axes are dense, else a contiguous copy. Strides of axes of one
-    element do not matter and are given as 0."""
-    if t is None:
-        return None, 0, 0
-    want = 1
-    for i in range(1, tail + 1):
-        if t.shape[-i] > 1 and t.stride(-i) != want:
-            t = t.contiguous()
+def _check(ts) -> int:
+    """The index of the one device that holds every tensor of ``ts``; refuses
+    CPU tensors and inputs that ask for gradients."""
+    idx = ts[0].get_device()
+    for t in ts:
+        if t.get_device() != idx or idx < 0:
+            _ops._require_cuda(*ts)
+            if len({t.device for t in ts}) > 1:
+                raise ValueError(f"tensors lie on different devices: {sorted({str(t.device) for t in ts})}")
             break
-        want *= t.shape[-i]
-    return t, t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t.requires_grad:
+                raise RuntimeError("this operator has no backward pass: call it under torch.no_grad() or "
+                                   "with detached tensors")
+    return idx
+
+
+def _rows(t: torch.Tensor, tail: int = 1):
+    """(tensor, its strides): ``t`` itself when its last ``tail`` axes are
+    dense, else a contiguous copy."""
+    s = t.stride()
+    if s[-1] != 1 or (tail == 2 and s[-2] != t.shape[-1]):
+        t = t.contiguous()
+        s = t.stride()
+    return t, s
+
+
+def _f32(t: torch.Tensor | None) -> torch.Tensor | None:
+    if t is None or (t.dtype is torch.float32 and t.is_contiguous()):
+        return t
+    return t.float().contiguous()
 
 
 def _sequences(x: torch.Tensor, cu_seqlens):
     """(number of sequences, tokens for the C call, cu_seqlens on the device)."""
-    _ops._check_varlen(x, None, cu_seqlens)
-    if x.shape[1] >= 1 << 31:
-        raise ValueError(f"{x.shape[1]} tokens are more than an int32 counts")
+    B, T = x.shape[0], x.shape[1]
+    if T >= 1 << 31:
+        raise ValueError(f"{T} tokens are more than an int32 counts")
     if cu_seqlens is None:
-        return x.shape[0], x.shape[1], None
-    if cu_seqlens.dim() != 1 or len(cu_seqlens) < 1:
+        return B, T, None
+    _ops._check_varlen(x, None, cu_seqlens)
+    if cu_seqlens.dim() != 1 or len(cu_seqlens) < 1 or cu_seqlens.is_floating_point():
         raise ValueError("cu_seqlens must be a vector of sequence offsets")
     if not cu_seqlens.is_cuda:
         c = cu_seqlens.to(torch.int64)
-        if int(c[0]) < 0 or int(c[-1]) > x.shape[1] or bool((c[1:] < c[:-1]).any()):
-            raise ValueError(f"cu_seqlens must ascend within [0, {x.shape[1]}]")
-    return len(cu_seqlens) - 1, x.shape[1], _ops._cu(cu_seqlens, x.device)
+        if int(c[0]) < 0 or int(c[-1]) > T or bool((c[1:] < c[:-1]).any()):
+            raise ValueError(f"cu_seqlens must ascend within [0, {T}]")
+    return len(cu_seqlens) - 1, T, _ops._cu(cu_seqlens, x.device)
 
 
-def _output(out: torch.Tensor | None, x: torch.Tensor, *inputs) -> torch.Tensor:
-    """A new contiguous tensor like x, or ``out`` once it is one that no input shares."""
-    if out is None:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous {tuple(x.shape)} {x.dtype} tensor on {x.device}")
+def _output(out: torch.Tensor, x: torch.Tensor, dtype, inputs) -> torch.Tensor:
+    """``out`` once it is a contiguous tensor like x that no input shares."""
+    if out.shape != x.shape or out.dtype != dtype or out.device != x.device or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous {tuple(x.shape)} {dtype} tensor on {x.device}")
     lo, hi = out.data_ptr(), out.data_ptr() + out.numel() * out.element_size()
     for t in inputs:
         if t is None or t.numel() == 0 or lo == hi:
@@ -90,21 +96,22 @@ def _output(out: torch.Tensor | None, x: torch.Tensor, *inputs) -> torch.Tensor:
     return out
 
 
-def _bank(bank: torch.Tensor, layer: int, tail: tuple[int, ...], dtype: torch.dtype, what: str):
-    if bank.dtype != dtype or not bank.is_contiguous() or bank.dim() != 2 + len(tail):
-        raise ValueError(f"the {what} bank must be a contiguous {dtype} tensor [L, S+1, "
-                         f"{', '.join(map(str, tail))}]")
-    if not 0 <= layer < bank.shape[0]:
-        raise IndexError(f"layer {layer} out of range [0, {bank.shape[0]})")
-    if tuple(bank.shape[2:]) != tail:
-        raise ValueError(f"bank rows of shape {tuple(bank.shape[2:])}, not {tail}")
-    return bank[layer]
+def _bank_rows(bank: torch.Tensor, layer: int, rows: int, cols: int, dtype: torch.dtype, what: str):
+    """(address, number of slots) of one layer of a family tensor [L, S+1, rows, cols]."""
+    if bank.dtype is not dtype or bank.dim() != 4 or not bank.is_contiguous():
+        raise ValueError(f"the {what} bank must be a contiguous {dtype} tensor [L, S+1, {rows}, {cols}]")
+    L, slots, r, c = bank.shape
+    if r != rows or c != cols:
+        raise ValueError(f"bank rows of shape ({r}, {c}), not ({rows}, {cols})")
+    if not 0 <= layer < L:
+        raise IndexError(f"layer {layer} out of range [0, {L})")
+    return bank.data_ptr() + layer * slots * rows * cols * bank.element_size(), slots
 
 
-def _slot_ids(slot_ids, num_slots: int, nseq: int, device) -> torch.Tensor:
-    ids = _ops.slot_ids_tensor(slot_ids, num_slots, device)
-    if ids.device != device:
-        raise ValueError(f"slot ids lie on {ids.device}, not {device}")
+def _slot_ids(slot_ids, num_slots: int, nseq: int, x: torch.Tensor) -> torch.Tensor:
+    ids = _ops.slot_ids_tensor(slot_ids, num_slots, x.device)
+    if ids.get_device() != x.get_device():
+        raise ValueError(f"slot ids lie on {ids.device}, not {x.device}")
     if ids.numel() != nseq:
         raise ValueError(f"{ids.numel()} slot ids for {nseq} sequences")
     return ids
@@ -114,27 +121,30 @@ def _slot_ids(slot_ids, num_slots: int, nseq: int, device) -> torch.Tensor:
 # short causal convolution
 # ---------------------------------------------------------------------------
 
-def _conv_args(x, weight, bias, activation):
-    _same_device(x, weight, bias)
-    _no_grad(x, weight, bias)
+def _conv_args(x, weight, bias, activation, *state):
+    """(device index, D, W, weight, bias, activation code), checked."""
+    idx = _check([t for t in (x, weight, bias, *state) if t is not None])
     if x.dim() != 3:
         raise ValueError(f"x must be [B, T, D], not {tuple(x.shape)}")
-    if x.dtype not in _ops._DTYPES:
-        raise ValueError(f"unsupported dtype {x.dtype}")
+    dtype, D = x.dtype, x.shape[2]
+    if dtype not in _ops._DTYPES:
+        raise ValueError(f"unsupported dtype {dtype}")
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation must be None or 'silu', not {activation!r}")
-    D = x.shape[2]
     if weight.dim() == 3 and weight.shape[1] == 1:  # a depthwise Conv1d's [D, 1, W]
         weight = weight[:, 0]
     if weight.dim() != 2 or weight.shape[0] != D:
         raise ValueError(f"weight must be [{D}, W], not {tuple(weight.shape)}")
-    if weight.shape[1] not in _WIDTHS:
-        raise ValueError(f"a width of {weight.shape[1]} is not supported (2, 3 or 4)")
-    if bias is not None and tuple(bias.shape) != (D,):
-        raise ValueError(f"bias must be [{D}], not {tuple(bias.shape)}")
-    weight = weight.to(x.dtype).contiguous()
-    bias = None if bias is None else bias.to(x.dtype).contiguous()
-    return weight, bias, _ACTIVATIONS[activation]
+    W = weight.shape[1]
+    if W not in _WIDTHS:
+        raise ValueError(f"a width of {W} is not supported (2, 3 or 4)")
+    if weight.dtype is not dtype or not weight.is_contiguous():
+        weight = weight.to(dtype).contiguous()
+    if bias is not None:
+        if bias.dim() != 1 or bias.shape[0] != D:
+            raise ValueError(f"bias must be [{D}], not {tuple(bias.shape)}")
+        bias = bias.to(dtype).contiguous()
+    return idx, D, W, weight, bias, _ACTIVATIONS[activation]
 
 
 def short_conv(x, weight, bias=None, activation: str | None = None, initial_state=None,
@@ -146,41 +156,35 @@ def short_conv(x, weight, bias=None, activation: str | None = None, initial_stat
     [N, W-1, D] in x's dtype holds the inputs before each sequence's first
     token, oldest first (None: zeros). Returns (o, final_state), the last W-1
     inputs of each sequence when ``output_final_state``, else None."""
-    weight, bias, act = _conv_args(x, weight, bias, activation)
-    _same_device(x, initial_state)
+    idx, D, W, weight, bias, act = _conv_args(x, weight, bias, activation, initial_state)
     N, T, cu = _sequences(x, cu_seqlens)
-    D, W = weight.shape
     if initial_state is not None:
-        _no_grad(initial_state)
         if tuple(initial_state.shape) != (N, W - 1, D):
             raise ValueError(f"initial_state must be {(N, W - 1, D)}, not {tuple(initial_state.shape)}")
         initial_state = initial_state.to(x.dtype).contiguous()
-    x, bs, ts = _rows(x)
-    o = _output(None, x)
+    x, (bs, ts, _) = _rows(x)
+    o = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     st = torch.empty(N, W - 1, D, dtype=x.dtype, device=x.device) if output_final_state else None
     p = _ops._ptr
-    with torch.cuda.device(x.device):
-        _lib.call("wkvm_short_conv", p(x), bs, ts, p(weight), p(bias), p(o), p(initial_state), p(st),
-                  p(cu), N, T, D, W, act, _ops._DTYPES[x.dtype], p(_ops.status_word(x.device)),
-                  _ops._stream(x.device))
+    _ops._launch("wkvm_short_conv", idx, p(x), bs, ts, p(weight), p(bias), p(o), p(initial_state), p(st), p(cu),
+                 N, T, D, W, act, _ops._DTYPES[x.dtype])
     return o, st
 
 
 def _conv_slots(x, weight, bank_conv, layer, slot_ids, bias, activation, cu_seqlens, out):
-    weight, bias, act = _conv_args(x, weight, bias, activation)
-    _same_device(x, bank_conv)
+    idx, D, W, weight, bias, act = _conv_args(x, weight, bias, activation, bank_conv)
     N, T, cu = _sequences(x, cu_seqlens)
-    D, W = weight.shape
-    layer_t = _bank(bank_conv, layer, (W - 1, D), x.dtype, "conv")
-    ids = _slot_ids(slot_ids, layer_t.shape[0], N, x.device)
-    x, bs, ts = _rows(x)
-    o = _output(out, x, x, layer_t)
+    rows, slots = _bank_rows(bank_conv, layer, W - 1, D, x.dtype, "conv")
+    ids = _slot_ids(slot_ids, slots, N, x)
+    x, (bs, ts, _) = _rows(x)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    else:
+        _output(out, x, x.dtype, (x, weight, bias, bank_conv))
     p = _ops._ptr
-    with torch.cuda.device(x.device):
-        _lib.call("wkvm_short_conv_slots", p(x), bs, ts, p(weight), p(bias), p(o), p(layer_t),
-                  layer_t.shape[0], p(ids), p(cu), N, T, D, W, act, _ops._DTYPES[x.dtype],
-                  p(_ops.status_word(x.device)), _ops._stream(x.device))
-    return o
+    _ops._launch("wkvm_short_conv_slots", idx, p(x), bs, ts, p(weight), p(bias), p(out), rows, slots, p(ids), p(cu),
+                 N, T, D, W, act, _ops._DTYPES[x.dtype])
+    return out
 
 
 def short_conv_decode_slots(x, weight, bank_conv: torch.Tensor, layer: int, slot_ids, bias=None,
@@ -204,53 +208,64 @@ def short_conv_prefill_slots(x, weight, bank_conv: torch.Tensor, layer: int, slo
 # ---------------------------------------------------------------------------
 
 class _Scan:
-    """Checked arguments of a selective scan in the C call's order."""
+    """Checked arguments of a selective scan, and its C call."""
 
-    def __init__(self, x, dt, A, B, C, D, z, dt_bias, cu_seqlens):
-        _same_device(x, dt, A, B, C, D, z, dt_bias)
-        _no_grad(x, dt, A, B, C, D, z, dt_bias)
-        if x.dim() != 3:
-            raise ValueError(f"x must be [B, T, D], not {tuple(x.shape)}")
-        d = x.shape[2]
-        for name, t in (("dt", dt), ("z", z)):
-            if t is not None and t.shape != x.shape:
-                raise ValueError(f"{name} must have x's shape {tuple(x.shape)}, not {tuple(t.shape)}")
+    __slots__ = ("idx", "dtype", "code", "nseq", "T", "d", "n", "g", "cu", "x", "inputs", "strides")
+
+    def __init__(self, x, dt, A, B, C, D, z, dt_bias, state, cu_seqlens):
+        self.idx = _check([t for t in (x, dt, A, B, C, D, z, dt_bias, state) if t is not None])
+        shape = x.shape
+        if len(shape) != 3:
+            raise ValueError(f"x must be [B, T, D], not {tuple(shape)}")
+        d = shape[2]
+        if dt.shape != shape:
+            raise ValueError(f"dt must have x's shape {tuple(shape)}, not {tuple(dt.shape)}")
+        if z is not None and z.shape != shape:
+            raise ValueError(f"z must have x's shape {tuple(shape)}, not {tuple(z.shape)}")
         if A.dim() != 2 or A.shape[0] != d:
             raise ValueError(f"A must be [{d}, N], not {tuple(A.shape)}")
         n = A.shape[1]
         if n not in _STATES:
             raise ValueError(f"{n} states per channel are not supported (8, 16, 32, 64 or 128)")
-        B, C = (t.unsqueeze(2) if t.dim() == 3 else t for t in (B, C))
+        grouped = B.dim() == 4
+        want = (shape[0], shape[1], B.shape[2], n) if grouped else (shape[0], shape[1], n)
         for name, t in (("B", B), ("C", C)):
-            if t.dim() != 4 or t.shape[:2] != x.shape[:2] or t.shape[3] != n or t.shape != B.shape:
-                raise ValueError(f"{name} must be [B, T, N] or [B, T, G, N] with N = {n}, "
+            if t.shape != want:
+                raise ValueError(f"{name} must be [B, T, N] or [B, T, G, N] with N = {n} and as many groups as B, "
                                  f"not {tuple(t.shape)}")
-        g = B.shape[2]
+        g = want[2] if grouped else 1
         if g < 1 or d % g:
             raise ValueError(f"{d} channels do not split into {g} groups")
         for name, t in (("D", D), ("dt_bias", dt_bias)):
-            if t is not None and tuple(t.shape) != (d,):
+            if t is not None and (t.dim() != 1 or t.shape[0] != d):
                 raise ValueError(f"{name} must be [{d}], not {tuple(t.shape)}")
-        self.dtype = x.dtype  # the output's
-        acts = [t for t in (x, dt, B, C, z) if t is not None]
-        if x.dtype not in _ops._DTYPES or any(t.dtype != x.dtype for t in acts):
+        self.dtype = dtype = x.dtype  # the output's
+        if (dtype not in _ops._DTYPES or dt.dtype is not dtype or B.dtype is not dtype or C.dtype is not dtype
+                or (z is not None and z.dtype is not dtype)):
             # mixed dtypes are widened to fp32 (lossless), as the other ops do
             x, dt, B, C, z = (None if t is None else t.float() for t in (x, dt, B, C, z))
         self.nseq, self.T, self.cu = _sequences(x, cu_seqlens)
-        self.x, self.shape = x, (self.nseq, self.T, d, n, g)
-        rows = [_rows(x), _rows(dt), _rows(z), _rows(B, 2), _rows(C, 2)]
-        x, dt, z, B, C = (r[0] for r in rows)
-        f32 = lambda t: None if t is None else t.float().contiguous()  # noqa: E731
-        # kept alive until the launch: some are copies made here
-        self.inputs = (x, dt, f32(A), B, C, f32(D), z, f32(dt_bias))
-        self.strides = (ctypes.c_int64 * 10)(*(s for r in rows for s in r[1:]))
+        self.d, self.n, self.g, self.code = d, n, g, _ops._DTYPES[x.dtype]
+        tail = 2 if grouped else 1
+        x, xs = _rows(x)
+        dt, ds = _rows(dt)
+        B, bs = _rows(B, tail)
+        C, cs = _rows(C, tail)
+        z, zs = (None, (0, 0)) if z is None else _rows(z)
+        self.x = x
+        # kept until the launch: some are copies made here
+        self.inputs = (x, dt, _f32(A), B, C, _f32(D), z, _f32(dt_bias))
+        self.strides = _Strides(xs[0], xs[1], ds[0], ds[1], zs[0], zs[1], bs[0], bs[1], cs[0], cs[1])
 
-    def call(self, entry, o, *state, softplus):
-        p, dev = _ops._ptr, self.x.device
-        with torch.cuda.device(dev):
-            _lib.call(entry, *(p(t) for t in self.inputs), p(o), self.strides, *state, p(self.cu),
-                      *self.shape, int(bool(softplus)), _ops._DTYPES[self.x.dtype],
-                      p(_ops.status_word(dev)), _ops._stream(dev))
+    def output(self):
+        return torch.empty(self.x.shape, dtype=self.x.dtype, device=self.x.device)
+
+    def call(self, entry, o, softplus, *state):
+        p = _ops._ptr
+        x, dt, A, B, C, D, z, bias = self.inputs
+        _ops._launch(entry, self.idx, x.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr(), p(D),
+                     p(z), p(bias), o.data_ptr(), self.strides, *state, p(self.cu), self.nseq, self.T, self.d,
+                     self.n, self.g, 1 if softplus else 0, self.code)
 
 
 def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus: bool = True,
@@ -266,32 +281,27 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus: bo
     D, dt_bias [D]; z, D and dt_bias optional. N in 8, 16, 32, 64, 128.
     States are fp32 [sequences, D, N]. Returns (o, final_state): o in x's
     dtype, final_state fp32 when ``output_final_state``, else None."""
-    a = _Scan(x, dt, A, B, C, D, z, dt_bias, cu_seqlens)
-    want = (a.nseq, a.shape[2], a.shape[3])
-    if initial_state is not None:
-        _same_device(x, initial_state)
-        _no_grad(initial_state)
-        if tuple(initial_state.shape) != want:
-            raise ValueError(f"initial_state must be {want}, not {tuple(initial_state.shape)}")
+    a = _Scan(x, dt, A, B, C, D, z, dt_bias, initial_state, cu_seqlens)
+    want = (a.nseq, a.d, a.n)
+    if initial_state is not None and tuple(initial_state.shape) != want:
+        raise ValueError(f"initial_state must be {want}, not {tuple(initial_state.shape)}")
     h0 = _ops._state(initial_state)
-    o = _output(None, a.x)
+    o = a.output()
     ht = torch.empty(want, dtype=torch.float32, device=x.device) if output_final_state else None
-    a.call("wkvm_selective_scan", o, _ops._ptr(h0), _ops._ptr(ht), softplus=dt_softplus)
+    a.call("wkvm_selective_scan", o, dt_softplus, _ops._ptr(h0), _ops._ptr(ht))
     return o.to(a.dtype), ht
 
 
 def _scan_slots(x, dt, A, B, C, bank_ssm, layer, slot_ids, D, z, dt_bias, dt_softplus, cu_seqlens, out):
-    a = _Scan(x, dt, A, B, C, D, z, dt_bias, cu_seqlens)
-    _same_device(x, bank_ssm)
-    layer_t = _bank(bank_ssm, layer, a.shape[2:4], torch.float32, "ssm")
-    ids = _slot_ids(slot_ids, layer_t.shape[0], a.nseq, x.device)
-    # a promoted call computes in fp32 and rounds into `out` afterwards
-    direct = a.x.dtype == a.dtype
+    a = _Scan(x, dt, A, B, C, D, z, dt_bias, bank_ssm, cu_seqlens)
+    rows, slots = _bank_rows(bank_ssm, layer, a.d, a.n, torch.float32, "ssm")
+    ids = _slot_ids(slot_ids, slots, a.nseq, x)
     if out is not None:
-        _output(out, x, *a.inputs, layer_t)
-    o = out if direct and out is not None else _output(None, a.x)
-    a.call("wkvm_selective_scan_slots", o, _ops._ptr(layer_t), layer_t.shape[0], _ops._ptr(ids),
-           softplus=dt_softplus)
+        _output(out, x, a.dtype, (x, *a.inputs, bank_ssm))
+    # a call of mixed dtypes computes in fp32 and rounds into `out` afterwards
+    direct = a.x.dtype is a.dtype
+    o = out if direct and out is not None else a.output()
+    a.call("wkvm_selective_scan_slots", o, dt_softplus, rows, slots, ids.data_ptr())
     if direct:
         return o
     return o.to(a.dtype) if out is None else out.copy_(o)
