@@ -367,6 +367,8 @@ int wkvm_selective_scan_slots(
     int32_t D, int32_t N, int32_t G, int32_t softplus, int32_t dtype,
     int32_t* status, wkvm_stream_t stream);
 
+enum { WKVM_SAMPLE_MAX_VOCAB = 393216 };
+
 /* Chooses one token for each of B rows of V logits (row_stride elements
  * apart) from a given uniform number u[b] in [0, 1). With m the row's
  * largest logit and w_i = exp((l_i - m) / temperature):
@@ -379,8 +381,8 @@ int wkvm_selective_scan_slots(
  * Ties go to the lowest ids. temperature <= 0 is greedy: the largest logit,
  * logprob 0. -inf and NaN logits are never chosen, +inf ones share the whole
  * mass, and a row with nothing to choose gives token -1 and logprob -inf.
- * Masses are fp64-accurate and summed in a fixed order: the same inputs give
- * the same token on every run. Each setting is a device array [B], or NULL
+ * Masses are rounded to V 2^-46 (65,536 logits; less for fewer) of the largest
+ * weight and summed exactly: the same inputs give the same token on every run. V is at most WKVM_SAMPLE_MAX_VOCAB. Each setting is a device array [B], or NULL
  * and the scalar beside it holds for every row. */
 int wkvm_sample_tokens(
     const void* logits, int64_t row_stride, const float* u, const float* temperature,

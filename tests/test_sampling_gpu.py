@@ -28,8 +28,11 @@ def _check(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     fin = np.isfinite(wlp)
     got = lp.double().cpu().numpy()
     assert (got[~fin] == wlp[~fin]).all()
-    # rounding to fp32, and 1e-11 of a mass
-    assert (np.abs(got[fin] - wlp[fin]) <= 2.0 ** -24 * np.abs(wlp[fin]) + 1e-11).all()
+    # rounding to fp32; weights to 2e-13; and the mass, a sum of V weights each rounded to a unit of 2^-s
+    # with s = min(52, 62 - ceil(log2 V)): off by V 2^-(s+1) at most, against a mass of at least 1
+    V = logits.shape[1]
+    s = min(52, 62 - math.ceil(math.log2(V)))
+    assert (np.abs(got[fin] - wlp[fin]) <= 2.0 ** -24 * np.abs(wlp[fin]) + 1e-12 + V * 2.0 ** -(s + 1)).all()
     return tok, lp
 
 

@@ -12,13 +12,34 @@
 // -inf and NaN logits are never kept; logits of +inf share the whole mass. A
 // row with nothing to keep gives token -1 and logprob -inf.
 //
-// Masses are fp64: where one token ends and the next begins moves by the
-// error of a running mass, and with 65,536 tokens an error of 1e-7 would
-// change about one row's token in two hundred.
+// Masses: where one token ends and the next begins moves by the error of a
+// running mass, and with 65,536 tokens an error of 1e-7 would change about
+// one row's token in two hundred. So weights are fp64 (2e-13), rounded once
+// to units of 2^-s and summed as 64-bit integers: sums are exact, whatever
+// the order, so atomics and every split over threads give the same result.
+// s is as large as V weights of 1 allow (46 for 65,536 logits): the rounding
+// moves a mass by V 2^-(s+1) at most, 2^-31 of the largest weight there.
+//
+// All three filters keep a prefix of the descending order, so what is kept is
+// one logit and a bound on the ids that equal it. A cluster of CTAs holds a
+// row in shared memory (logits are read from HBM once) and finds that bound
+// by histograms of counts (top-k) or masses (top-p) over the logits above a
+// lower bound, then finishes on a sorted list of at most kCap candidates in
+// one CTA. Only a larger set is narrowed by further histograms and drawn from
+// by a pass over the whole row. 65,536 logits cost 2.1e6 fp64 operations in
+// exponentials, which with the passes over shared memory and the cluster's
+// barriers bound it; HBM does not.
+#include <cooperative_groups.h>
+
+#include <atomic>
+
 #include "common.cuh"
 
 namespace wkvm {
 namespace {
+
+namespace cg = cooperative_groups;
+typedef unsigned long long u64;
 
 struct SampleArgs {
   const void* logits;
@@ -30,178 +51,668 @@ struct SampleArgs {
   int32_t top_k0;
   int64_t* token;
   float* logprob;
-  int32_t B, V;
-  int* status;
+  int32_t V;
+  int32_t slice;  // logits of one CTA, a multiple of kNT
+  double shift;   // 2^(52-s): adding it leaves a weight's units in the low bits
+  bool vec;       // rows start on 16 bytes
 };
 
-// Ascending unsigned order of floats; NaN and -inf become 0 (never kept).
+constexpr int kNT = 512, kWarps = kNT / 32;
+constexpr int kBins = 1024;
+constexpr int kCap = 1024;        // candidates one CTA sorts
+constexpr int kMaxCtas = 8;       // CTAs of a row (portable cluster size)
+
+// Ascending unsigned order of floats; -inf is 0 and never kept (NaN and -0
+// are gone by then).
 __device__ __forceinline__ uint32_t key_of(float x) {
-  if (!(x > -INFINITY)) return 0u;
-  const uint32_t b = __float_as_uint(x + 0.0f);  // -0 sorts as +0
+  if (x == -INFINITY) return 0u;
+  const uint32_t b = __float_as_uint(x);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 __device__ __forceinline__ float value_of(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
 
-constexpr int kThreads = 1024;
+// 2^t for -64 <= t <= 0: the power series of e^(f ln 2), |f| <= 1/2, to degree
+// 10 (truncation 2.2e-13), times 2^n through the exponent.
+__device__ __forceinline__ double exp2_neg(double t) {
+  const double magic = 6755399441055744.0;  // 1.5 * 2^52: rounds to an integer
+  const double r = t + magic;
+  const int n = __double2loint(r);
+  const double f = t - (r - magic);
+  double p = 7.0549116208011233e-09;
+  p = fma(p, f, 1.0178086009239699e-07);
+  p = fma(p, f, 1.3215486790144309e-06);
+  p = fma(p, f, 1.5252733804059841e-05);
+  p = fma(p, f, 1.5403530393381609e-04);
+  p = fma(p, f, 1.3333558146428443e-03);
+  p = fma(p, f, 9.6181291076284772e-03);
+  p = fma(p, f, 5.5504108664821580e-02);
+  p = fma(p, f, 2.4022650695910072e-01);
+  p = fma(p, f, 6.9314718055994531e-01);
+  p = fma(p, f, 1.0);
+  return __hiloint2double(__double2hiint(p) + (n << 20), __double2loint(p));
+}
 
-template <typename V, typename F>
-__device__ V block_sum(V x, V* scratch, F) {
+struct Found {          // what a level of a selection found, the same in every CTA
+  int bin;              // the bin with the boundary; -1: everything is kept
+  uint32_t above, in;   // candidates in the bins above it, and in it
+  u64 mass_above, mass_in;
+};
+
+// Shared memory of a CTA ahead of its slice of logits. Fields named peer_* are
+// written by the other CTAs of the cluster, [rank] by rank.
+struct Shared {
+  uint32_t cnt[kBins];              // histogram: counts
+  uint32_t mass_lo[kBins], mass_hi[kBins];  // and masses
+  u64 list[kCap];                   // candidates: ~key << 32 | id, ascending = the descending order
+  u64 weight[kCap];
+  u64 warp_sum[kWarps];
+  uint32_t warp_u32[3][kWarps];
+  uint32_t peer_max[kMaxCtas], peer_warp[kMaxCtas], peer_thread[kMaxCtas];
+  uint32_t peer_lo[kMaxCtas], peer_hi[kMaxCtas], peer_cnt[kMaxCtas];
+  u64 peer_mass[kMaxCtas], peer_total[kMaxCtas];
+  Found found;
+  uint32_t n_list;
+  uint32_t tau;                     // the last kept key
+  int32_t limit;                    // ids below it are kept among its equals
+  int32_t first;                    // greedy
+};
+
+struct Row {
+  Shared* s;
+  const float* vals;
+  int rank, ctas, tid, lane, warp, slice, base;  // base: the slice's first id
+  double m, c;       // maximum; log2(e) / temperature
+  double shift;      // of units(), a power of two >= 1
+  uint32_t mkey;
+  uint32_t tau;      // kept: key > tau, or key == tau and id < limit
+  int32_t limit;
+
+  __device__ double weight(float l) const {
+    const double t = ((double)l - m) * c;
+    if (__float_as_uint(l) == __float_as_uint((float)m)) return 1.0;
+    return t > -54.0 ? exp2_neg(t) : 0.0;  // less than half a unit (NaN: a maximum of inf)
+  }
+  __device__ u64 units(double w) const {
+    return (u64)(__double_as_longlong(w + shift) - __double_as_longlong(shift));
+  }
+  __device__ double weight_of(u64 z) const { return (double)z * (shift * 0x1p-52); }
+  __device__ u64 mass(float l) const { return units(weight(l)); }
+  __device__ bool kept(uint32_t k, int id) const { return k > tau || (k == tau && id < limit); }
+
+  template <typename T>
+  __device__ T warp_add(T x) const {
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
+    for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
+    return x;
+  }
+  // Sum over the CTA, returned to every thread.
+  __device__ u64 block_add(u64 x) const {
+    x = warp_add(x);
+    __syncthreads();
+    if (lane == 0) s->warp_sum[warp] = x;
+    __syncthreads();
+    u64 t = 0;
+    for (int i = 0; i < kWarps; ++i) t += s->warp_sum[i];
+    return t;
+  }
+  __device__ Shared* peer(int r) const { return cg::this_cluster().map_shared_rank(s, r); }
+  __device__ static void sync() { cg::this_cluster().sync(); }  // the row's CTAs
+};
+
+// A level's bins: keys [lo, hi] into kBins bins, the largest first. Linear in
+// the logit where that is safe, else linear in the key; any monotone map does.
+struct Bins {
+  uint32_t lo, hi;
+  float top, scale;  // scale 0: linear in the key
+  u64 step;          // ceil(2^32 bins / keys)
+  __device__ Bins(uint32_t l, uint32_t h) : lo(l), hi(h), top(value_of(h)), scale(0.f), step(0) {
+    const float range = top - value_of(l);
+    if (range > 1e-30f && range < 1e30f)
+      scale = kBins / range;
+    else
+      step = ((u64)kBins << 32) / ((u64)(h - l) + 1);
+  }
+  __device__ int operator()(float l, uint32_t k) const {
+    const int b = scale > 0.f ? (int)((top - l) * scale) : (int)(((u64)(hi - k) * step) >> 32);
+    return b < kBins - 1 ? b : kBins - 1;
+  }
+};
+
+// One level: histogram of the kept candidates with keys in [b.lo, b.hi], and
+// the first bin at which above + the running count (or mass) reaches the goal.
+// `rest`: mass of what is kept below b.lo joins the total, and the goal is
+// share times that total (first level of top-p). Two cluster barriers.
+template <bool MASS>
+__device__ void level(Row& r, const Bins& b, uint32_t above, u64 mass_above, double goal, bool rest,
+                      double share, u64* total) {
+  Shared* s = r.s;
+  for (int i = r.tid; i < kBins; i += kNT) {
+    s->cnt[i] = 0;
+    if (MASS) s->mass_lo[i] = s->mass_hi[i] = 0;
+  }
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = x;
+  u64 all = 0;
+  for (int i = r.tid; i < r.slice; i += kNT) {
+    const float l = r.vals[i];
+    const uint32_t k = key_of(l);
+    if (k > b.hi || (k < b.lo && !rest) || !r.kept(k, r.base + i)) continue;
+    u64 w = 0;
+    if (MASS) w = r.mass(l);
+    if (MASS && rest) all += w;
+    if (k < b.lo) continue;
+    const int bin = b(l, k);
+    atomicAdd(&s->cnt[bin], 1u);
+    if (MASS) {
+      const uint32_t lo = (uint32_t)w, old = atomicAdd(&s->mass_lo[bin], lo);
+      const uint32_t hi = (uint32_t)(w >> 32) + (old + lo < old);
+      if (hi) atomicAdd(&s->mass_hi[bin], hi);
+    }
+  }
+  if (MASS && rest) {
+    all = r.block_add(all);
+    if (r.tid < r.ctas) r.peer(r.tid)->peer_total[r.rank] = all;
+  }
+  r.sync();
+  if (MASS && rest) {
+    all = 0;
+    for (int i = 0; i < r.ctas; ++i) all += s->peer_total[i];
+    *total = all;
+    goal = share * (double)all;
+  }
+  if (r.rank == 0) {
+    // two neighbouring bins a thread, summed over the cluster
+    uint32_t c[2] = {0, 0};
+    u64 m[2] = {0, 0};
+    for (int p = 0; p < r.ctas; ++p) {
+      const Shared* o = r.peer(p);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        c[j] += o->cnt[2 * r.tid + j];
+        if (MASS) m[j] += o->mass_lo[2 * r.tid + j] + ((u64)o->mass_hi[2 * r.tid + j] << 32);
+      }
+    }
+    uint32_t cs = c[0] + c[1];
+    u64 ms = m[0] + m[1];
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const uint32_t cu = __shfl_up_sync(0xffffffffu, cs, off);
+      const u64 mu = __shfl_up_sync(0xffffffffu, ms, off);
+      if (r.lane >= off) {
+        cs += cu;
+        ms += mu;
+      }
+    }
+    __syncthreads();
+    if (r.lane == 31) {
+      s->warp_u32[0][r.warp] = cs;
+      s->warp_sum[r.warp] = ms;
+    }
+    if (r.tid == 0) s->found.bin = -1;
+    __syncthreads();
+    uint32_t cb = above;
+    u64 mb = mass_above;
+    for (int i = 0; i < r.warp; ++i) {
+      cb += s->warp_u32[0][i];
+      mb += s->warp_sum[i];
+    }
+    cb += cs - c[0] - c[1];  // what is above this thread's bins
+    mb += ms - m[0] - m[1];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const bool before = MASS ? (double)mb < goal : (double)cb < goal;
+      const bool reached = MASS ? (double)(mb + m[j]) >= goal : (double)(cb + c[j]) >= goal;
+      if (c[j] && before && reached) s->found = {2 * r.tid + j, cb, c[j], mb, m[j]};
+      cb += c[j];
+      mb += m[j];
+    }
+    __syncthreads();
+    // to every CTA
+    const int words = sizeof(Found) / 4;
+    for (int i = r.tid; i < words * (r.ctas - 1); i += kNT)
+      reinterpret_cast<uint32_t*>(&r.peer(1 + i / words)->found)[i % words] =
+          reinterpret_cast<const uint32_t*>(&s->found)[i % words];
+    if (r.tid == 0) s->n_list = 0;
+  }
+  r.sync();
+}
+
+// Kept candidates whose bin is `bin` (or above it too) go to the first CTA's list.
+__device__ void gather(Row& r, const Bins& b, int bin, bool above_too) {
+  Shared* first = r.peer(0);
+  for (int i = r.tid; i < r.slice; i += kNT) {
+    const float l = r.vals[i];
+    const uint32_t k = key_of(l);
+    if (k < b.lo || !r.kept(k, r.base + i)) continue;
+    if (k > b.hi) {
+      if (!above_too) continue;
+    } else {
+      const int at = b(l, k);
+      if (above_too ? at > bin : at != bin) continue;
+    }
+    const uint32_t slot = atomicAdd(&first->n_list, 1u);
+    if (slot < kCap) first->list[slot] = ((u64)~k << 32) | (uint32_t)(r.base + i);
+  }
+  r.sync();
+}
+
+// Sorts the first n entries of the list ascending (one CTA, n <= kCap).
+__device__ void sort_list(Row& r, int n) {
+  Shared* s = r.s;
+  int size = 2;
+  while (size < n) size *= 2;
+  for (int i = n + r.tid; i < size; i += kNT) s->list[i] = ~0ull;
   __syncthreads();
-  V s = 0;
-  for (int i = 0; i < kThreads / 32; ++i) s += scratch[i];
-  return s;
+  for (int k = 2; k <= size; k *= 2)
+    for (int j = k / 2; j > 0; j /= 2) {
+      for (int t = r.tid; t < size / 2; t += kNT) {
+        const int a = 2 * t - (t & (j - 1)), b = a + j;
+        const u64 x = s->list[a], y = s->list[b];
+        if ((x > y) == ((a & k) == 0)) {
+          s->list[a] = y;
+          s->list[b] = x;
+        }
+      }
+      __syncthreads();
+    }
+}
+
+// Inclusive sums of weight[0, n) in place (one CTA, two neighbours a thread).
+__device__ void scan_weights(Row& r, int n) {
+  Shared* s = r.s;
+  const int i = 2 * r.tid;
+  const u64 a = i < n ? s->weight[i] : 0, b = i + 1 < n ? s->weight[i + 1] : 0;
+  u64 x = a + b;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const u64 up = __shfl_up_sync(0xffffffffu, x, off);
+    if (r.lane >= off) x += up;
+  }
+  __syncthreads();
+  if (r.lane == 31) s->warp_sum[r.warp] = x;
+  __syncthreads();
+  for (int w = 0; w < r.warp; ++w) x += s->warp_sum[w];
+  if (i < n) s->weight[i] = x - b;
+  if (i + 1 < n) s->weight[i + 1] = x;
+  __syncthreads();
+}
+
+__device__ __forceinline__ uint32_t list_key(u64 e) { return ~(uint32_t)(e >> 32); }
+
+// The row's end on the list: n candidates, of which the first k are in play.
+// total: the mass top-p takes its share of (0: of these k).
+__device__ void finish_list(Row& r, int n, int k, double tp, double mp, double u, u64 total,
+                            int64_t* token, float* logprob) {
+  Shared* s = r.s;
+  sort_list(r, n);
+  if (k < n) n = k;
+  auto weigh = [&](int i) { return r.weight(value_of(list_key(s->list[i]))); };
+  if (tp < 1.0) {
+    for (int i = r.tid; i < n; i += kNT) s->weight[i] = r.units(weigh(i));
+    __syncthreads();
+    scan_weights(r, n);
+    const double goal = tp * (double)(total ? total : s->weight[n - 1]);
+    // entry i stays while the mass before it is short of the goal
+    uint32_t stay = 0;
+    for (int i = r.tid; i < n; i += kNT) stay += i == 0 || (double)s->weight[i - 1] < goal;
+    n = (int)r.block_add(stay);
+  }
+  if (mp > 0.0) {
+    uint32_t stay = 0;
+    for (int i = r.tid; i < n; i += kNT) stay += i == 0 || weigh(i) >= mp || list_key(s->list[i]) == r.mkey;
+    n = (int)r.block_add(stay);
+  }
+  // draw in order of ids
+  for (int i = r.tid; i < n; i += kNT) {
+    const u64 e = s->list[i];
+    s->list[i] = (e << 32) | (e >> 32);
+  }
+  __syncthreads();
+  sort_list(r, n);
+  auto by_id = [&](int i) { return r.weight(value_of(~(uint32_t)s->list[i])); };
+  for (int i = r.tid; i < n; i += kNT) s->weight[i] = r.units(by_id(i));
+  __syncthreads();
+  scan_weights(r, n);
+  const u64 z = s->weight[n - 1];
+  double goal = u * (double)z;
+  if (!(goal < (double)z)) goal = (double)(z - 1);
+  for (int i = r.tid; i < n; i += kNT) {
+    const u64 before = i ? s->weight[i - 1] : 0;
+    if (s->weight[i] > before && (double)s->weight[i] > goal && !((double)before > goal)) {
+      *token = (int64_t)(s->list[i] >> 32);
+      *logprob = (float)log(by_id(i) / r.weight_of(z));
+    }
+  }
+}
+
+// Keeps, of the kept candidates that equal `key`, the `want` lowest ids.
+__device__ void limit_ties(Row& r, uint32_t key, uint32_t want) {
+  Shared* s = r.s;
+  const int per = r.slice / kWarps, i0 = r.warp * per;
+  uint32_t c = 0;
+  for (int i = i0 + r.lane; i < i0 + per; i += 32) c += key_of(r.vals[i]) == key && r.kept(key, r.base + i);
+  c = r.warp_add(c);
+  __syncthreads();
+  if (r.lane == 0) s->warp_u32[0][r.warp] = c;
+  __syncthreads();
+  if (r.tid < r.ctas) {
+    uint32_t t = 0;
+    for (int w = 0; w < kWarps; ++w) t += s->warp_u32[0][w];
+    r.peer(r.tid)->peer_cnt[r.rank] = t;
+  }
+  r.sync();
+  uint32_t before = 0;
+  for (int p = 0; p < r.rank; ++p) before += s->peer_cnt[p];
+  for (int w = 0; w < r.warp; ++w) before += s->warp_u32[0][w];
+  if (before < want && before + s->warp_u32[0][r.warp] >= want) {  // one warp of the cluster
+    for (int i = i0; i < i0 + per; i += 32) {
+      const bool is = key_of(r.vals[i + r.lane]) == key && r.kept(key, r.base + i + r.lane);
+      const uint32_t b = __ballot_sync(0xffffffffu, is);
+      if (before + __popc(b) < want) {
+        before += __popc(b);
+        continue;
+      }
+      const bool last = is && before + __popc(b & ((2u << r.lane) - 1)) == want;
+      if (last)
+        for (int p = 0; p < r.ctas; ++p) r.peer(p)->limit = r.base + i + r.lane + 1;
+      break;
+    }
+  }
+  r.sync();
+  r.tau = key;
+  r.limit = s->limit;
+}
+
+// Narrows what is kept to the first candidates in descending order whose
+// count reaches `goal` (or whose mass reaches tp of the mass of all kept).
+// Returns true when the row was finished on the list.
+template <bool MASS>
+__device__ bool select(Row& r, uint32_t lo, double goal, int k, double tp, double mp, double u,
+                       int64_t* token, float* logprob) {
+  Shared* s = r.s;
+  Bins b(lo, r.mkey);
+  uint32_t above = 0;
+  u64 mass_above = 0, total = 0;
+  for (bool first = true;; first = false) {
+    level<MASS>(r, b, above, mass_above, goal, MASS && first, tp, &total);
+    if (MASS && first) goal = tp * (double)total;
+    Found f = s->found;
+    // counts: fewer than the goal in all. masses: a goal that no mass is short
+    // of (a share of nothing), the top alone is kept
+    if (f.bin < 0) {
+      if (!MASS) return false;
+      limit_ties(r, r.mkey, 1);
+      return false;
+    }
+    if (f.above + f.in <= kCap) {
+      gather(r, b, f.bin, true);
+      if (r.rank == 0) finish_list(r, (int)(f.above + f.in), MASS ? INT32_MAX : k, tp, mp, u, total, token, logprob);
+      return true;
+    }
+    if (f.in <= kCap) {
+      gather(r, b, f.bin, false);
+      if (r.rank == 0) {
+        const int n = (int)f.in;
+        sort_list(r, n);
+        for (int i = r.tid; i < n; i += kNT) s->weight[i] = MASS ? r.mass(value_of(list_key(s->list[i]))) : 1;
+        __syncthreads();
+        scan_weights(r, n);
+        const u64 base = MASS ? f.mass_above : f.above;
+        for (int i = r.tid; i < n; i += kNT) {
+          const double before = (double)(base + (i ? s->weight[i - 1] : 0));
+          if (before < goal && ((double)(base + s->weight[i]) >= goal || i == n - 1))
+            for (int p = 0; p < r.ctas; ++p) {
+              r.peer(p)->tau = list_key(s->list[i]);
+              r.peer(p)->limit = (int32_t)(uint32_t)s->list[i] + 1;
+            }
+        }
+      }
+      r.sync();
+      r.tau = s->tau;
+      r.limit = s->limit;
+      return false;
+    }
+    // too many: their smallest and largest key bound the next level
+    uint32_t kl = 0xffffffffu, kh = 0;
+    for (int i = r.tid; i < r.slice; i += kNT) {
+      const float l = r.vals[i];
+      const uint32_t q = key_of(l);
+      if (q < b.lo || q > b.hi || !r.kept(q, r.base + i) || b(l, q) != f.bin) continue;
+      kl = min(kl, q);
+      kh = max(kh, q);
+    }
+    kl = __reduce_min_sync(0xffffffffu, kl);
+    kh = __reduce_max_sync(0xffffffffu, kh);
+    __syncthreads();
+    if (r.lane == 0) {
+      s->warp_u32[0][r.warp] = kl;
+      s->warp_u32[1][r.warp] = kh;
+    }
+    __syncthreads();
+    if (r.tid < r.ctas) {
+      for (int w = 0; w < kWarps; ++w) {
+        kl = min(kl, s->warp_u32[0][w]);
+        kh = max(kh, s->warp_u32[1][w]);
+      }
+      r.peer(r.tid)->peer_lo[r.rank] = kl;
+      r.peer(r.tid)->peer_hi[r.rank] = kh;
+    }
+    r.sync();
+    for (int p = 0; p < r.ctas; ++p) {
+      kl = min(kl, s->peer_lo[p]);
+      kh = max(kh, s->peer_hi[p]);
+    }
+    if (kl == kh) {  // equal logits: as many as it takes
+      uint32_t want = (uint32_t)(goal - (double)f.above);
+      if (MASS) {
+        const u64 w = r.mass(value_of(kl));
+        want = (uint32_t)fmin((goal - (double)f.mass_above) / (double)w, (double)(f.in - 1)) ;
+        while (want > 0 && (double)(f.mass_above + (want - 1) * w) >= goal) --want;
+        while (want < f.in && (double)(f.mass_above + want * w) < goal) ++want;
+      }
+      limit_ties(r, kl, want);
+      return false;
+    }
+    above = f.above;
+    mass_above = f.mass_above;
+    b = Bins(kl, kh);
+  }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs p) {
-  __shared__ double sd[kThreads / 32];
-  __shared__ int si[kThreads / 32];
-  __shared__ int s_token;
-  const int b = blockIdx.x, tid = threadIdx.x, V = p.V;
-  const T* row = static_cast<const T*>(p.logits) + b * p.row_stride;
+__global__ void __launch_bounds__(kNT) sample_kernel(SampleArgs p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  Row r;
+  Shared* s = r.s = reinterpret_cast<Shared*>(smem);
+  float* vals = reinterpret_cast<float*>(smem + sizeof(Shared));
+  r.vals = vals;
+  r.rank = (int)cg::this_cluster().block_rank();
+  r.ctas = (int)cg::this_cluster().num_blocks();
+  r.tid = threadIdx.x;
+  r.lane = r.tid & 31;
+  r.warp = r.tid >> 5;
+  r.slice = p.slice;
+  r.base = r.rank * p.slice;
+  r.tau = 0;  // key 0 is never kept
+  r.limit = 0;
+  const int b = blockIdx.x / r.ctas;
+  const T* row = static_cast<const T*>(p.logits) + b * p.row_stride + r.base;
+  const int n = min(p.slice, p.V - r.base);  // may be <= 0
+
+  // ---- the slice into shared memory, and its maximum
+  uint32_t mine = 0;
+  auto put = [&](int i, float v) {
+    v = v > -INFINITY ? v + 0.f : -INFINITY;  // NaN counts as -inf, -0 as 0
+    vals[i] = v;
+    mine = max(mine, key_of(v));
+  };
+  constexpr int kVec = 16 / sizeof(T);
+  const int whole = p.vec ? max(n, 0) / kVec * kVec : 0;
+  for (int i = r.tid * kVec; i < whole; i += kNT * kVec) {
+    const uint4 q = *reinterpret_cast<const uint4*>(row + i);
+    const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) put(i + j, to_f32(e[j]));
+  }
+  for (int i = whole + r.tid; i < p.slice; i += kNT) put(i, i < n ? to_f32(row[i]) : -INFINITY);
+
+  const double u = p.u[b];
   float temp = p.temperature ? p.temperature[b] : p.temperature0;
   int k = p.top_k ? p.top_k[b] : p.top_k0;
   const double tp = p.top_p ? p.top_p[b] : p.top_p0, mp = p.min_p ? p.min_p[b] : p.min_p0;
-  const double u = p.u[b];
-  if (!(temp > 0.f)) { temp = 1.f; k = 1; }
-  const double inv_t = 1.0 / (double)temp;
-  auto key = [&](int i) { return key_of(to_f32(row[i])); };
-  auto isum = [&](int x) { return block_sum<int>(x, si, 0); };
-  auto dsum = [&](double x) { return block_sum<double>(x, sd, 0); };
+  if (!(temp > 0.f)) k = 1;
 
-  // the largest key and how many logits can be kept at all
-  uint32_t mk = 0;
-  int n = 0;
-  for (int i = tid; i < V; i += kThreads) {
-    const uint32_t q = key(i);
-    mk = max(mk, q);
-    n += q != 0;
+  // maximum of the row; the least maximum over the warps and over the threads
+  // (of that many disjoint sets) bounds as many largest logits from below
+  const uint32_t wmax = __reduce_max_sync(0xffffffffu, mine), wmin = __reduce_min_sync(0xffffffffu, mine);
+  if (r.lane == 0) {
+    s->warp_u32[0][r.warp] = wmax;
+    s->warp_u32[1][r.warp] = wmin;
   }
-  n = isum(n);
-  __shared__ unsigned s_mk;
-  if (tid == 0) { s_mk = 0; s_token = -1; }
+  if (r.tid == 0) s->first = INT32_MAX;
   __syncthreads();
-  atomicMax(&s_mk, mk);
-  __syncthreads();
-  mk = s_mk;
-  if (n == 0) {
-    if (tid == 0) { p.token[b] = -1; p.logprob[b] = -INFINITY; }
+  if (r.tid < r.ctas) {
+    uint32_t mx = 0, mw = 0xffffffffu, mt = 0xffffffffu;
+    for (int w = 0; w < kWarps; ++w) {
+      mx = max(mx, s->warp_u32[0][w]);
+      mw = min(mw, s->warp_u32[0][w]);
+      mt = min(mt, s->warp_u32[1][w]);
+    }
+    Shared* o = r.peer(r.tid);
+    o->peer_max[r.rank] = mx;
+    o->peer_warp[r.rank] = mw;
+    o->peer_thread[r.rank] = mt;
+  }
+  r.sync();
+  uint32_t least_w = 0xffffffffu, least_t = 0xffffffffu;
+  r.mkey = 0;
+  for (int i = 0; i < r.ctas; ++i) {
+    r.mkey = max(r.mkey, s->peer_max[i]);
+    least_w = min(least_w, s->peer_warp[i]);
+    least_t = min(least_t, s->peer_thread[i]);
+  }
+  if (r.mkey == 0) {
+    if (r.rank == 0 && r.tid == 0) {
+      p.token[b] = -1;
+      p.logprob[b] = -INFINITY;
+    }
     return;
   }
-  const double m = value_of(mk);
-  auto weight = [&](uint32_t q) -> double {
-    if (q == 0) return 0.0;
-    if (q == mk) return 1.0;
-    if (isinf(m)) return 0.0;
-    return exp(((double)value_of(q) - m) * inv_t);
-  };
+  r.m = value_of(r.mkey);
+  r.c = 1.4426950408889634 / (double)temp;
+  r.shift = p.shift;
 
-  // kept: key > tau, or key == tau and id < lim (always a prefix of the
-  // descending order)
-  uint32_t tau = 0;
-  int lim = 0;  // key 0 is never kept
-  auto kept = [&](uint32_t q, int i) { return q > tau || (q == tau && i < lim); };
-  auto limit_ids = [&](uint32_t key_eq, int budget) {  // id bound that keeps `budget` ties
-    int lo = 0, hi = V;
-    while (lo < hi) {
-      const int mid = lo + (hi - lo) / 2;
-      int c = 0;
-      for (int i = tid; i < mid; i += kThreads) c += key(i) == key_eq;
-      c = isum(c);
-      if (c >= budget) hi = mid; else lo = mid + 1;
+  if (k == 1) {  // the lowest id of the largest logit
+    int at = INT32_MAX;
+    for (int i = r.tid; i < p.slice; i += kNT)
+      if (key_of(vals[i]) == r.mkey) {
+        at = i + r.base;
+        break;
+      }
+    at = __reduce_min_sync(0xffffffffu, at);
+    if (r.lane == 0 && at != INT32_MAX) atomicMin(&r.peer(0)->first, at);
+    r.sync();
+    if (r.rank == 0 && r.tid == 0) {
+      p.token[b] = s->first;
+      p.logprob[b] = 0.f;
     }
-    return lo;
-  };
-  if (k > 0 && k < n) {
-    uint32_t lo = 1, hi = mk;  // largest key with at least k keys >= it
-    while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo) / 2 + 1;
-      int c = 0;
-      for (int i = tid; i < V; i += kThreads) c += key(i) >= mid;
-      c = isum(c);
-      if (c >= k) lo = mid; else hi = mid - 1;
-    }
-    int above = 0;
-    for (int i = tid; i < V; i += kThreads) above += key(i) > lo;
-    above = isum(above);
-    lim = limit_ids(lo, k - above);
-    tau = lo;
+    return;
   }
-  auto mass_from = [&](uint32_t from) {  // mass of what is kept with key >= from
-    double s = 0;
-    for (int i = tid; i < V; i += kThreads) {
-      const uint32_t q = key(i);
-      if (q >= from && kept(q, i)) s += weight(q);
-    }
-    return dsum(s);
-  };
+  if (k > 0 && k < p.V) {
+    uint32_t lo = k <= r.ctas * kWarps ? least_w : k <= r.ctas * kNT ? least_t : 0u;
+    if (lo == 0) lo = 1;  // an empty set among them: no bound
+    if (select<false>(r, lo, (double)k, k, tp, mp, u, p.token + b, p.logprob + b)) return;
+  }
   if (tp < 1.0) {
-    const double goal = tp * mass_from(0);
-    uint32_t lo = 1, hi = mk;
-    while (lo < hi) {  // largest key with mass >= goal at or above it
-      const uint32_t mid = lo + (hi - lo) / 2 + 1;
-      if (mass_from(mid) >= goal) lo = mid; else hi = mid - 1;
-    }
-    const double above = lo == 0xffffffffu ? 0.0 : mass_from(lo + 1);
-    int ties = 0;
-    for (int i = tid; i < V; i += kThreads) {
-      const uint32_t q = key(i);
-      ties += q == lo && kept(q, i);
-    }
-    ties = isum(ties);
-    const double w = weight(lo);
-    int take = 1;
-    while (take < ties && above + take * w < goal) ++take;
-    lim = limit_ids(lo, take);
-    tau = lo;
+    // tokens of weight below (1 - p) / 2V hold less than 1 - p of the mass, as
+    // the largest alone weighs 1: the boundary lies above them
+    const double eps = (1.0 - tp) / (2.0 * (double)p.V);
+    const float bound = (float)(r.m + log2(eps) / r.c * 1.0001 - fabs(r.m) * 3e-7);
+    uint32_t lo = bound > -INFINITY ? key_of(bound) : 1u;
+    lo = max(min(lo, r.mkey), 1u);
+    if (select<true>(r, lo, 0.0, k, tp, mp, u, p.token + b, p.logprob + b)) return;
   }
-  // draw: contiguous ids per thread
-  const int per = (V + kThreads - 1) / kThreads;
-  const int i0 = min(V, tid * per), i1 = min(V, i0 + per);
-  auto share = [&](int i) {
-    const uint32_t q = key(i);
-    if (!kept(q, i)) return 0.0;
-    const double w = weight(q);
-    return w >= mp || q == mk ? w : 0.0;
+
+  // ---- draw from the whole row: masses of contiguous blocks, one per warp
+  const int per = p.slice / kWarps, i0 = r.warp * per;
+  // logits this low have w < mp for certain
+  const float low = mp > 0.0 ? (float)(r.m + log2(mp) / r.c * 1.0001 - fabs(r.m) * 3e-7) : -INFINITY;
+  auto share = [&](int i, double* w) -> u64 {
+    const float l = vals[i];
+    const uint32_t q = key_of(l);
+    if (q != r.mkey && (l < low || !r.kept(q, r.base + i))) return 0;
+    if (q == r.mkey && !r.kept(q, r.base + i)) return 0;
+    *w = r.weight(l);
+    return *w >= mp || q == r.mkey ? r.units(*w) : 0;
   };
-  double mine = 0;
-  for (int i = i0; i < i1; ++i) mine += share(i);
-  __shared__ double s_mass[kThreads];
-  s_mass[tid] = mine;
+  u64 sum = 0;
+  double w;
+  for (int i = i0 + r.lane; i < i0 + per; i += 32) sum += share(i, &w);
+  sum = r.warp_add(sum);
   __syncthreads();
-  if (tid == 0) {
-    double z = 0;
-    for (int t = 0; t < kThreads; ++t) z += s_mass[t];
-    const double goal = u * z;
-    double c = 0, wt = 0;
-    int tok = -1;
-    for (int t = 0; t < kThreads && (tok < 0 || c <= goal); ++t) {
-      if (s_mass[t] == 0.0) continue;
-      if (c + s_mass[t] <= goal && t * per + per < V) {
-        bool later = false;
-        for (int r = t + 1; r < kThreads; ++r) later |= s_mass[r] > 0.0;
-        if (later) { c += s_mass[t]; continue; }
-      }
-      const int a0 = min(V, t * per), a1 = min(V, a0 + per);
-      for (int i = a0; i < a1; ++i) {
-        const double w = share(i);
-        if (w == 0.0) continue;
-        tok = i;
-        wt = w;
-        c += w;
-        if (c > goal) break;
-      }
-      if (c > goal) break;
-    }
-    p.token[b] = tok;
-    p.logprob[b] = (float)log(wt / z);
+  if (r.lane == 0) s->warp_sum[r.warp] = sum;
+  __syncthreads();
+  if (r.tid < r.ctas) {
+    u64 t = 0;
+    for (int i = 0; i < kWarps; ++i) t += s->warp_sum[i];
+    r.peer(r.tid)->peer_mass[r.rank] = t;
   }
+  r.sync();
+  u64 z = 0, before = 0;
+  for (int i = 0; i < r.ctas; ++i) {
+    if (i < r.rank) before += s->peer_mass[i];
+    z += s->peer_mass[i];
+  }
+  for (int i = 0; i < r.warp; ++i) before += s->warp_sum[i];
+  double goal = u * (double)z;
+  if (!(goal < (double)z)) goal = (double)(z - 1);
+  // the one warp in whose block the running mass passes the goal
+  if (sum == 0 || (double)before > goal || !((double)(before + sum) > goal)) return;
+  for (int i = i0; i < i0 + per; i += 32) {
+    w = 0.0;
+    const u64 own = share(i + r.lane, &w);
+    u64 x = own;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const u64 up = __shfl_up_sync(0xffffffffu, x, off);
+      if (r.lane >= off) x += up;
+    }
+    const bool hit = own && (double)(before + x) > goal;
+    const uint32_t any = __ballot_sync(0xffffffffu, hit);
+    if (any) {
+      if (r.lane == __ffs(any) - 1) {
+        p.token[b] = r.base + i + r.lane;
+        p.logprob[b] = (float)log(w / r.weight_of(z));
+      }
+      return;
+    }
+    before += __shfl_sync(0xffffffffu, x, 31);
+  }
+}
+
+template <typename T>
+int launch(const SampleArgs& a, int B, int ctas, cudaStream_t st) {
+  const int bytes = (int)sizeof(Shared) + a.slice * 4;
+  static std::atomic<uint64_t> done{0};  // a bit per device: the shared-memory limit is raised
+  int dev = 0;
+  WKVM_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev >= 64 || !(done.load(std::memory_order_acquire) >> dev & 1)) {
+    WKVM_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 << 10));
+    if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((int64_t)B * ctas));
+  cfg.blockDim = dim3(kNT);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, sample_kernel<T>, a) == cudaSuccess ? WKVM_OK : WKVM_ERR_CUDA;
 }
 
 }  // namespace
@@ -213,18 +724,28 @@ extern "C" int wkvm_sample_tokens(const void* logits, int64_t row_stride, const 
                                   int32_t top_k0, float top_p0, float min_p0, int64_t* tokens,
                                   float* logprobs, int32_t B, int32_t V, int32_t dtype,
                                   int32_t* status, wkvm_stream_t stream) {
+  (void)status;  // nothing in a row can be wrong on the device
   if (B < 0 || V <= 0) return WKVM_ERR_INVALID_ARG;
   if (dtype != WKVM_DTYPE_F32 && dtype != WKVM_DTYPE_BF16 && dtype != WKVM_DTYPE_F16)
     return WKVM_ERR_DTYPE;
+  if (V > WKVM_SAMPLE_MAX_VOCAB) return WKVM_ERR_SHAPE;
   if (B == 0) return WKVM_OK;
   if (!logits || !u || !tokens || !logprobs) return WKVM_ERR_INVALID_ARG;
-  wkvm::SampleArgs a{logits, row_stride, u, temperature, top_p, min_p, top_k, temperature0,
-                     top_p0, min_p0, top_k0, tokens, logprobs, B, V, status};
+  // about 8,192 logits a CTA: sixteen a thread
+  int ctas = 1;
+  while (ctas < wkvm::kMaxCtas && V > ctas * 8192) ctas *= 2;
+  if ((int64_t)B * ctas > INT32_MAX) return WKVM_ERR_SHAPE;
+  const int64_t es = dtype == WKVM_DTYPE_F32 ? 4 : 2;
+  const int slice = ((V + ctas - 1) / ctas + wkvm::kNT - 1) / wkvm::kNT * wkvm::kNT;
+  const bool vec = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && (B == 1 || row_stride * es % 16 == 0);
+  double shift = 1.0;  // s = min(52, 62 - ceil(log2 V))
+  for (int64_t v = 1 << 10; v < V; v *= 2) shift *= 2.0;
+  wkvm::SampleArgs a{logits, row_stride, u, temperature, top_p, min_p, top_k, temperature0, top_p0,
+                     min_p0, top_k0, tokens, logprobs, V, slice, shift, vec};
   cudaStream_t st = (cudaStream_t)stream;
   switch (dtype) {
-    case WKVM_DTYPE_F32: wkvm::sample_kernel<float><<<B, wkvm::kThreads, 0, st>>>(a); break;
-    case WKVM_DTYPE_BF16: wkvm::sample_kernel<__nv_bfloat16><<<B, wkvm::kThreads, 0, st>>>(a); break;
-    default: wkvm::sample_kernel<__half><<<B, wkvm::kThreads, 0, st>>>(a); break;
+    case WKVM_DTYPE_F32: return wkvm::launch<float>(a, B, ctas, st);
+    case WKVM_DTYPE_BF16: return wkvm::launch<__nv_bfloat16>(a, B, ctas, st);
+    default: return wkvm::launch<__half>(a, B, ctas, st);
   }
-  return cudaGetLastError() == cudaSuccess ? WKVM_OK : WKVM_ERR_CUDA;
 }

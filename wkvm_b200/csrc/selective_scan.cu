@@ -110,13 +110,15 @@ __global__ void __launch_bounds__(kRowThreads) scan_rows_kernel(ScanArgs p) {
 // Tile kernel, for prompts. T D N exponentials (16 a clock and SM) bound it:
 // 16 states give 4.65e12 / s against 8 bytes of activations per 16 of them.
 //
-// One CTA walks one sequence for CB channels, kTT tokens at a time. Each
-// thread keeps NS states of one channel; the L = N / NS threads of a channel
-// leave their partial sums of C h in shared memory and the thread that owns
-// the output element adds them. What is per (token, channel) - softplus, the
+// One CTA walks one sequence for CB channels, TT tokens at a time. A thread
+// keeps NS states of CH channels; the L = N / NS threads of a channel leave
+// their partial sums of C h in shared memory and the thread that owns the
+// output element adds them. What is per (token, channel) - softplus, the
 // skip, the gate, conversions - is done once by the owner of the element, not
-// by the L threads: they read (delta, delta x) pairs. Inputs of the next tile
-// are in registers while this one runs.
+// by the L threads: they read (delta, delta x) pairs. Shared memory gives
+// 128 bytes a clock however many lanes read the same word, so a thread's
+// share of B and C (kept in the inputs' dtype) is read once for its CH
+// channels. Inputs of the next tile are in registers while this one runs.
 //
 // Few rows (a long prompt alone, few channels): the CTAs of a cluster split
 // the sequence's tiles between them. Each first runs its part from a zero
@@ -124,8 +126,6 @@ __global__ void __launch_bounds__(kRowThreads) scan_rows_kernel(ScanArgs p) {
 // the part's whole decay, A being constant), then takes the parts before it
 // from its peers' shared memory and runs its part again from its true start.
 // ---------------------------------------------------------------------------
-constexpr int kTT = 32;
-
 typedef unsigned long long f32x2;
 __device__ __forceinline__ f32x2 pack2(float x, float y) {
   f32x2 r;
@@ -148,39 +148,116 @@ __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
   return r;
 }
 
-template <typename T, int V> struct alignas(sizeof(T) * V) Raw { T e[V]; };
-
-// V elements at p, of which the first `n` exist (the others read as zero).
-// vec: p is aligned to the whole vector and n is 0 or at least V.
-template <typename T, int V>
-__device__ __forceinline__ Raw<T, V> load_raw(const T* p, int n, bool vec) {
-  Raw<T, V> r;
-  if (vec && n >= V) return *reinterpret_cast<const Raw<T, V>*>(p);
-#pragma unroll
-  for (int i = 0; i < V; ++i) r.e[i] = i < n ? p[i] : from_f32<T>(0.f);
+// V elements as they lie in memory, held as words: elements of 16 bits kept
+// apart would be taken apart, and so waited for, right after the load.
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 
+template <typename T, int V>
+struct Raw {
+  static constexpr int kBytes = sizeof(T) * V, kWords = (kBytes + 3) / 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ float f32(int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[i]);
+    } else {
+      const uint16_t h = (uint16_t)(w[i / 2] >> (16 * (i % 2)));
+      return to_f32(*reinterpret_cast<const T*>(&h));
+    }
+  }
+  __device__ __forceinline__ void set(int i, float x) {
+    const T t = from_f32<T>(x);
+    if constexpr (sizeof(T) == 4) {
+      w[i] = *reinterpret_cast<const uint32_t*>(&t);
+    } else {
+      const uint32_t h = *reinterpret_cast<const uint16_t*>(&t);
+      w[i / 2] = i % 2 ? (w[i / 2] & 0xffffu) | h << 16 : h;
+    }
+  }
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void move(Raw<T, V>* dst, const Raw<T, V>* src) {  // one access each way
+  constexpr int B = Raw<T, V>::kBytes;
+  if constexpr (B >= 16) {
+#pragma unroll
+    for (int i = 0; i < B / 16; ++i) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
+  } else if constexpr (B == 8) {
+    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(src);
+  } else if constexpr (B == 4) {
+    *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
+  } else {
+    *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(src);
+  }
+}
+
+// V elements at p, of which the first `n` exist (the others read as zero).
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> load_some(const T* p, int n) {
+  Raw<T, V> r;
+#pragma unroll
+  for (int i = 0; i < Raw<T, V>::kWords; ++i) r.w[i] = 0;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if (i >= n) continue;
+    if constexpr (sizeof(T) == 4)
+      r.w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    else
+      r.w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[i] << (16 * (i % 2));
+  }
+  return r;
+}
+
+// V elements from global to shared memory, zeros where there are none (n <= 0).
+// vec: src is aligned to the whole vector and n is at most 0 or at least V;
+// the copy is then asynchronous, for copies_done() to wait for.
+template <typename T, int V>
+__device__ __forceinline__ void copy_in(T* dst, const T* src, const T* safe, int n, bool vec) {
+  if (vec) {
+    const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+    const T* from = n > 0 ? src : safe;
+    const int size = n > 0 ? Raw<T, V>::kBytes : 0;
+    if constexpr (Raw<T, V>::kBytes == 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(from), "r"(size) : "memory");
+    else
+      asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(from), "n"(Raw<T, V>::kBytes), "r"(size) : "memory");
+  } else {
+    const Raw<T, V> r = load_some<T, V>(src, n);
+    move<T, V>(reinterpret_cast<Raw<T, V>*>(dst), &r);
+  }
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 constexpr int min_i(int a, int b) { return a < b ? a : b; }
 
-template <int N, int NS, int NT>
+// 4 floats of padding behind every 32 keep 16-byte accesses of neighbouring
+// threads off each other's banks
+__host__ __device__ constexpr int padded(int i) { return i + (i >> 5) * 4; }
+
+// N states; NP pairs of channels and NS states a thread; NT threads; tiles of
+// TT tokens.
+template <typename T, int N, int NP, int NS, int NT, int TT>
 struct Tile {
-  static constexpr int L = N / NS;                  // threads of a channel
-  static constexpr int CB = NT / L;                 // channels of a CTA
-  static constexpr int TP = 4 / NS;                 // tokens in one 16-byte read of B or C
-  static constexpr int EPT = kTT * CB / NT;         // elements of x a thread owns
-  static constexpr int VE = min_i(EPT, 4), RV = EPT / VE;
-  static constexpr int BPT = kTT * N / NT;          // elements of B a thread loads
-  static constexpr int VB = min_i(BPT, 4), RB = BPT / VB;
-  static constexpr int YROW = NT + NT / 8;          // 4 floats of padding every 32: no bank conflicts
-  // shared memory, in floats
-  static constexpr int oD = 0;                      // [kTT / TP][CB][TP] (delta, delta x)
-  static constexpr int oB = oD + 2 * kTT * CB;      // [kTT / TP][L][TP][NS]
-  static constexpr int oC = oB + kTT * N;
-  static constexpr int oY = oC + kTT * N;           // [kTT][YROW] partial sums
-  static constexpr int oH = oY + kTT * YROW;        // cluster: final states [NS][NT], step sums [NT]
-  static constexpr int bytes(bool cluster) { return 4 * (oH + (cluster ? (NS + 1) * NT : 0)); }
-  static_assert(EPT >= 1 && BPT >= 1 && CB >= 1, "tile too small for the block");
+  static constexpr int L = N / NS;                        // threads of a channel
+  static constexpr int CBP = NT / L, CB = 2 * CBP * NP;   // a thread's pairs: ch + j CBP, j < NP
+  static constexpr int EPT = TT * CB / NT;                // elements of x a thread owns
+  static constexpr int VE = min_i(EPT, 16 / (int)sizeof(T)), RV = EPT / VE;
+  static constexpr int BPT = TT * N / NT;                 // elements of B a thread loads
+  static constexpr int VB = min_i(BPT, 16 / (int)sizeof(T)), RB = BPT / VB;
+  static constexpr int DROW = padded(2 * CB), YROW = padded(2 * NP * NT);
+  // shared memory, in bytes
+  static constexpr int XB = sizeof(T) * TT * CB, BB = sizeof(T) * TT * N;
+  static constexpr int oD = 0;                      // [TT][pair] (delta, delta, delta x, delta x)
+  static constexpr int oY = oD + 4 * TT * DROW;     // [TT][pair][L][2] partial sums
+  static constexpr int oX = oY + 4 * TT * YROW;     // two stages of x, dt, z [TT][CB] and B, C [TT][N]
+  static constexpr int kStage = 3 * XB + 2 * BB;
+  static constexpr int oP = oX + 2 * kStage;        // dt_bias and D of the channels
+  static constexpr int oH = oP + 8 * CB;            // cluster: final states, step sums
+  static constexpr int bytes(bool cluster) { return oH + (cluster ? 8 * NP * (NS + 1) * NT : 0); }
+  static_assert(EPT >= 2 && BPT >= 2 && TT * NT % CB == 0 && XB % 16 == 0 && BB % 16 == 0, "tile too small for the block");
 };
 
 struct TileArgs {
@@ -191,12 +268,18 @@ struct TileArgs {
   bool longest_first;
 };
 
-template <typename T, int N, int NS, int NT, bool CLUSTER>
+template <typename T, int N, int NP, int NS, int NT, int TT, bool CLUSTER>
 __global__ void __launch_bounds__(NT) scan_tiles_kernel(TileArgs q) {
-  using K = Tile<N, NS, NT>;
-  constexpr int L = K::L, CB = K::CB, TP = K::TP, VE = K::VE, RV = K::RV, VB = K::VB, RB = K::RB;
-  constexpr int CBV = CB / VE;
-  extern __shared__ __align__(16) float sm[];
+  using K = Tile<T, N, NP, NS, NT, TT>;
+  constexpr int L = K::L, CB = K::CB, CBP = K::CBP, VE = K::VE, RV = K::RV, VB = K::VB, RB = K::RB;
+  constexpr int CBV = CB / VE, TS = NT / CBV;
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* sD = reinterpret_cast<float*>(smem + K::oD);
+  float* sY = reinterpret_cast<float*>(smem + K::oY);
+  float* sP = reinterpret_cast<float*>(smem + K::oP);
+  auto meet = [] {
+    if constexpr (NT == 32) __syncwarp(); else __syncthreads();
+  };
   const ScanArgs& p = q.s;
   const int tid = threadIdx.x, lane = tid % L, ch = tid / L;
   const int part = CLUSTER ? (int)(blockIdx.x % q.parts) : 0;
@@ -221,7 +304,7 @@ __global__ void __launch_bounds__(NT) scan_tiles_kernel(TileArgs q) {
       }
       if (rank == n) s_n = i;
     }
-    __syncthreads();
+    meet();
     n = s_n;
   }
   int64_t row;
@@ -235,30 +318,27 @@ __global__ void __launch_bounds__(NT) scan_tiles_kernel(TileArgs q) {
     return;
   }
 
-  // ---- this thread's states and its channel's A
-  const bool on = ch < cn;
-  const int64_t hoff = (row * p.D + c0 + (on ? ch : 0)) * N + lane * NS;
-  f32x2 h[NS / 2], a[NS / 2];
-  float hs[NS];
+  // ---- this thread's states and their A, two channels in a register pair
+  f32x2 h[NP][NS], a[NP][NS];
 #pragma unroll
-  for (int i = 0; i < NS; ++i) hs[i] = p.h_in ? p.h_in[hoff + i] : 0.f;
+  for (int j = 0; j < NP; ++j) {
+    const int c = 2 * (ch + j * CBP);
+    const float* ap = p.A + (int64_t)(c0 + c) * N + lane * NS;
+    const float* hp = p.h_in + (row * p.D + c0 + c) * N + lane * NS;
 #pragma unroll
-  for (int i = 0; i < NS / 2; ++i) {
-    const float* ap = p.A + (int64_t)(c0 + (on ? ch : 0)) * N + lane * NS + 2 * i;
-    a[i] = pack2(scaled(ap[0]), scaled(ap[1]));
-    h[i] = pack2(hs[2 * i], hs[2 * i + 1]);
+    for (int i = 0; i < NS; ++i) {
+      a[j][i] = pack2(c < cn ? scaled(ap[i]) : 0.f, c + 1 < cn ? scaled(ap[N + i]) : 0.f);
+      h[j][i] = pack2(p.h_in && c < cn ? hp[i] : 0.f, p.h_in && c + 1 < cn ? hp[N + i] : 0.f);
+    }
   }
 
   // ---- the elements of a tile this thread owns: channels ce..ce+VE-1 of
   //      tokens te + r * TS
   const int te = tid / CBV, ce = (tid % CBV) * VE;
-  constexpr int TS = NT / CBV;
   const int nv = cn - ce;  // channels of the vector that exist
-  float bias[VE], skip[VE];
-#pragma unroll
-  for (int i = 0; i < VE; ++i) {
-    bias[i] = p.bias && i < nv ? p.bias[c0 + ce + i] : 0.f;
-    skip[i] = p.skip && i < nv ? p.skip[c0 + ce + i] : 0.f;
+  for (int i = tid; i < CB; i += NT) {
+    sP[i] = p.bias && i < cn ? p.bias[c0 + i] : 0.f;
+    sP[CB + i] = p.skip && i < cn ? p.skip[c0 + i] : 0.f;
   }
   const T* xp = static_cast<const T*>(p.x.p) + act_row(p.seqs, p.x, n, sp.bos) + c0 + ce;
   const T* dp = static_cast<const T*>(p.dt.p) + act_row(p.seqs, p.dt, n, sp.bos) + c0 + ce;
@@ -267,125 +347,158 @@ __global__ void __launch_bounds__(NT) scan_tiles_kernel(TileArgs q) {
   const T* cp = static_cast<const T*>(p.C.p) + act_row(p.seqs, p.C, n, sp.bos) + g * N;
   T* op = static_cast<T*>(p.o) + sp.bos * p.D + c0 + ce;
 
-  Raw<T, VE> rx[RV], rd[RV], rz[RV];
-  Raw<T, VB> rb[RB], rc[RB];
-  auto fetch = [&](int64_t t0, bool emit) {
+  // A thread copies in the elements it owns and is their only reader, so it
+  // waits for its own copies alone; B and C, read by all, are also behind the
+  // barrier ahead of the main loop.
+  auto fetch = [&](int64_t t0, int stage, bool emit) {
+    T* s = reinterpret_cast<T*>(smem + K::oX + stage * K::kStage);
 #pragma unroll
     for (int r = 0; r < RV; ++r) {
       const int64_t t = t0 + te + r * TS;
-      const int k = t < sp.len ? nv : 0;
-      rx[r] = load_raw<T, VE>(xp + t * p.x.ts, k, q.vec_x);
-      rd[r] = load_raw<T, VE>(dp + t * p.dt.ts, k, q.vec_x);
-      if (emit && zp) rz[r] = load_raw<T, VE>(zp + t * p.z.ts, k, q.vec_x);
+      const int k = t < sp.len ? nv : 0, at = (te + r * TS) * CB + ce;
+      copy_in<T, VE>(s + at, xp + t * p.x.ts, xp, k, q.vec_x);
+      copy_in<T, VE>(s + TT * CB + at, dp + t * p.dt.ts, dp, k, q.vec_x);
+      if (emit && zp) copy_in<T, VE>(s + 2 * TT * CB + at, zp + t * p.z.ts, zp, k, q.vec_x);
     }
+    s += 3 * TT * CB;
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
       const int e = (r * NT + tid) * VB;
       const int64_t t = t0 + e / N;
       const int k = t < sp.len ? VB : 0;
-      rb[r] = load_raw<T, VB>(bp + t * p.B.ts + e % N, k, q.vec_b);
-      if (emit) rc[r] = load_raw<T, VB>(cp + t * p.C.ts + e % N, k, q.vec_b);
+      copy_in<T, VB>(s + e, bp + t * p.B.ts + e % N, bp, k, q.vec_b);
+      if (emit) copy_in<T, VB>(s + TT * N + e, cp + t * p.C.ts + e % N, cp, k, q.vec_b);
     }
   };
 
-  float steps = 0.f;  // sum of delta over the part (first pass of a cluster)
+  f32x2 steps[NP];  // sums of delta over the part (first pass of a cluster)
+#pragma unroll
+  for (int j = 0; j < NP; ++j) steps[j] = 0;
   auto run = [&](int64_t t0, int64_t t1, bool emit) {
     if (t0 >= t1) return;
-    fetch(t0, emit);
-    for (; t0 < t1; t0 += kTT) {
-      Raw<T, VE> cx[RV], cz[RV];
+    fetch(t0, 0, emit);
+    meet();  // sP; the tiles of an earlier run
+    for (int stage = 0; t0 < t1; t0 += TT, stage ^= 1) {
+      const T* sX = reinterpret_cast<const T*>(smem + K::oX + stage * K::kStage);
+      const T* sB = sX + 3 * TT * CB;
+      const T* sC = sB + TT * N;
+      copies_done();
 #pragma unroll
       for (int r = 0; r < RV; ++r) {
-        cx[r] = rx[r];
-        cz[r] = rz[r];
         const int t = te + r * TS;
         const bool live = t0 + t < sp.len;
-        float* dst = sm + K::oD + 2 * ((t / TP) * CB * TP + (t % TP));
+        float* dst = sD + t * K::DROW + padded(2 * ce);
+        Raw<T, VE> rx, rd;
+        move<T, VE>(&rx, reinterpret_cast<const Raw<T, VE>*>(sX + t * CB + ce));
+        move<T, VE>(&rd, reinterpret_cast<const Raw<T, VE>*>(sX + TT * CB + t * CB + ce));
 #pragma unroll
-        for (int i = 0; i < VE; ++i) {
-          float d = to_f32(rd[r].e[i]) + bias[i];
-          if (p.softplus) d = softplus(d);
-          if (!live) d = 0.f;  // decay 1, input 0
-          *reinterpret_cast<float2*>(dst + 2 * TP * (ce + i)) = make_float2(d, live ? d * to_f32(cx[r].e[i]) : 0.f);
+        for (int i = 0; i < VE; i += 2) {
+          const float2 bias = *reinterpret_cast<const float2*>(sP + ce + i);
+          float d0 = rd.f32(i) + bias.x, d1 = rd.f32(i + 1) + bias.y;
+          if (p.softplus) {
+            d0 = softplus(d0);
+            d1 = softplus(d1);
+          }
+          if (!live) d0 = d1 = 0.f;  // behind the end: decay 1, and x is 0: input 0
+          *reinterpret_cast<float4*>(dst + 2 * i) = make_float4(d0, d1, d0 * rx.f32(i), d1 * rx.f32(i + 1));
         }
       }
+      meet();
+      if (t0 + TT < t1) fetch(t0 + TT, stage ^ 1, emit);
+      const int live = (int)(sp.len - t0 < TT ? sp.len - t0 : TT);
+      // operands of the next U tokens are read before this U are computed, and
+      // the U partial sums stored after it: a store between would hold back
+      // every later read
+      constexpr int U = NP * NS <= 4 ? 2 : 1;
+      Raw<T, NS> nb[U], nc[U];
+      ulonglong2 nd[U][NP];
+      auto operands = [&](int t0) {
 #pragma unroll
-      for (int r = 0; r < RB; ++r) {
-        const int e = (r * NT + tid) * VB;
+        for (int u = 0; u < U; ++u) {
+          const int t = t0 + u;
+          move<T, NS>(&nb[u], reinterpret_cast<const Raw<T, NS>*>(sB + t * N + lane * NS));
+          if (emit) move<T, NS>(&nc[u], reinterpret_cast<const Raw<T, NS>*>(sC + t * N + lane * NS));
 #pragma unroll
-        for (int i = 0; i < VB; ++i) {
-          const int t = (e + i) / N, s = (e + i) % N;
-          const int at = (((t / TP) * L + s / NS) * TP + t % TP) * NS + s % NS;
-          sm[K::oB + at] = to_f32(rb[r].e[i]);
-          if (emit) sm[K::oC + at] = to_f32(rc[r].e[i]);
+          for (int j = 0; j < NP; ++j)
+            nd[u][j] = *reinterpret_cast<const ulonglong2*>(sD + t * K::DROW + padded(4 * (ch + j * CBP)));
         }
-      }
-      __syncthreads();
-      if (t0 + kTT < t1) fetch(t0 + kTT, emit);
-      const int live = (int)(sp.len - t0 < kTT ? sp.len - t0 : kTT);
-      const float* sD = sm + K::oD + 2 * TP * ch;
-      const float* sB = sm + K::oB + 4 * lane;
-      const float* sC = sm + K::oC + 4 * lane;
-      float* sY = sm + K::oY + tid + (tid >> 5) * 4;
-      for (int tb = 0; tb < live; tb += 8) {
+      };
+      operands(0);
+#pragma unroll(4 / U)
+      for (int tb = 0; tb < live; tb += U) {
+        Raw<T, NS> kb[U], kc[U];
+        ulonglong2 kd[U][NP];
+        f32x2 y[U][NP];
 #pragma unroll
-        for (int u = 0; u < 8; u += TP) {
-          const int t = tb + u;
-          float dd[2 * TP];
-          if constexpr (TP == 2)
-            *reinterpret_cast<float4*>(dd) = *reinterpret_cast<const float4*>(sD + 2 * CB * t);
-          else
-            *reinterpret_cast<float2*>(dd) = *reinterpret_cast<const float2*>(sD + 2 * CB * t);
-          const ulonglong2 bb = *reinterpret_cast<const ulonglong2*>(sB + (t / TP) * 4 * L);
-          ulonglong2 cc = make_ulonglong2(0, 0);
-          if (emit) cc = *reinterpret_cast<const ulonglong2*>(sC + (t / TP) * 4 * L);
+        for (int u = 0; u < U; ++u) {
+          kb[u] = nb[u];
+          if (emit) kc[u] = nc[u];
 #pragma unroll
-          for (int v = 0; v < TP; ++v) {
-            const f32x2 d2 = pack2(dd[2 * v], dd[2 * v]), x2 = pack2(dd[2 * v + 1], dd[2 * v + 1]);
-            f32x2 y2 = 0;
+          for (int j = 0; j < NP; ++j) kd[u][j] = nd[u][j];
+        }
+        if (tb + U < TT) operands(tb + U);
 #pragma unroll
-            for (int i = 0; i < NS / 2; ++i) {
-              const f32x2 b2 = (v * (NS / 2) + i) ? bb.y : bb.x, c2 = (v * (NS / 2) + i) ? cc.y : cc.x;
-              const float2 e = unpack2(mul2(a[i], d2));
-              h[i] = fma2(pack2(ex2(e.x), ex2(e.y)), h[i], mul2(x2, b2));
-              y2 = i ? fma2(h[i], c2, y2) : mul2(h[i], c2);
-            }
-            if (emit) {
-              const float2 y = unpack2(y2);
-              sY[(t + v) * K::YROW] = y.x + y.y;
-            } else {
-              steps += dd[2 * v];
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+          for (int i = 0; i < NS; ++i) {
+            const f32x2 b2 = pack2(kb[u].f32(i), kb[u].f32(i));
+            const f32x2 c2 = emit ? pack2(kc[u].f32(i), kc[u].f32(i)) : 0;
+#pragma unroll
+            for (int j = 0; j < NP; ++j) {
+              const float2 e = unpack2(mul2(a[j][i], kd[u][j].x));
+              h[j][i] = fma2(pack2(ex2(e.x), ex2(e.y)), h[j][i], mul2(kd[u][j].y, b2));
+              if (emit) y[u][j] = i ? fma2(h[j][i], c2, y[u][j]) : mul2(h[j][i], c2);
             }
           }
+          if (!emit) {
+#pragma unroll
+            for (int j = 0; j < NP; ++j) steps[j] = add2(steps[j], kd[u][j].x);
+          }
+        }
+        if (emit) {
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < NP; ++j)
+              *reinterpret_cast<f32x2*>(sY + (tb + u) * K::YROW + padded(2 * j * NT) + padded(2 * tid)) = y[u][j];
         }
       }
-      __syncthreads();
+      meet();
       if (!emit) continue;
 #pragma unroll
       for (int r = 0; r < RV; ++r) {
         const int t = te + r * TS;
-        if (t0 + t >= sp.len) continue;
-        const float* src = sm + K::oY + t * K::YROW + ce * L + ((ce * L) >> 5) * 4;
-        Raw<T, VE> out;
+        if (t0 + t >= sp.len || nv <= 0) continue;
+        const float* src = sY + t * K::YROW + padded(ce * L);
+        Raw<T, VE> rx, rz, out;
+        move<T, VE>(&rx, reinterpret_cast<const Raw<T, VE>*>(sX + t * CB + ce));
+        if (zp) move<T, VE>(&rz, reinterpret_cast<const Raw<T, VE>*>(sX + 2 * TT * CB + t * CB + ce));
 #pragma unroll
-        for (int i = 0; i < VE; ++i) {
-          float y = 0.f;
+        for (int i = 0; i < VE; i += 2) {
+          const float2 skip = *reinterpret_cast<const float2*>(sP + CB + ce + i);
+          float2 y = make_float2(0.f, 0.f);
 #pragma unroll
-          for (int j = 0; j < L; j += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(src + (i * L + j) + ((i * L + j) >> 5) * 4);
-            y += (f.x + f.y) + (f.z + f.w);
+          for (int j = 0; j < L; ++j) {
+            const float2 f = *reinterpret_cast<const float2*>(src + padded(i * L + 2 * j));
+            y.x += f.x;
+            y.y += f.y;
           }
-          y = fmaf(skip[i], to_f32(cx[r].e[i]), y);
-          if (zp) y *= silu<sizeof(T) == 4>(to_f32(cz[r].e[i]));
-          out.e[i] = from_f32<T>(y);
+          y.x = fmaf(skip.x, rx.f32(i), y.x);
+          y.y = fmaf(skip.y, rx.f32(i + 1), y.y);
+          if (zp) {
+            y.x *= silu<sizeof(T) == 4>(rz.f32(i));
+            y.y *= silu<sizeof(T) == 4>(rz.f32(i + 1));
+          }
+          out.set(i, y.x);
+          out.set(i + 1, y.y);
         }
         T* dst = op + (t0 + t) * p.D;
-        if (q.vec_x && nv >= VE) {
-          *reinterpret_cast<Raw<T, VE>*>(dst) = out;
+        if (q.vec_x) {
+          move<T, VE>(reinterpret_cast<Raw<T, VE>*>(dst), &out);
         } else {
 #pragma unroll
           for (int i = 0; i < VE; ++i)
-            if (i < nv) dst[i] = out.e[i];
+            if (i < nv) dst[i] = from_f32<T>(out.f32(i));
         }
       }
     }
@@ -394,48 +507,58 @@ __global__ void __launch_bounds__(NT) scan_tiles_kernel(TileArgs q) {
   if constexpr (CLUSTER) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
-    const int64_t tiles = (sp.len + kTT - 1) / kTT, each = (tiles + q.parts - 1) / q.parts * kTT;
+    const int64_t tiles = (sp.len + TT - 1) / TT, each = (tiles + q.parts - 1) / q.parts * TT;
     const int64_t b0 = part * each < sp.len ? part * each : sp.len;
     const int64_t b1 = b0 + each < sp.len ? b0 + each : sp.len;
-    f32x2 start[NS / 2];
+    f32x2 start[NP][NS];
 #pragma unroll
-    for (int i = 0; i < NS / 2; ++i) {
-      start[i] = h[i];
-      h[i] = 0;
-    }
+    for (int j = 0; j < NP; ++j)
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        start[j][i] = h[j][i];
+        h[j][i] = 0;
+      }
     if (part + 1 < q.parts) run(b0, b1, false);  // nobody follows the last part
-    float* sH = sm + K::oH;
+    f32x2* sH = reinterpret_cast<f32x2*>(smem + K::oH);
 #pragma unroll
-    for (int i = 0; i < NS / 2; ++i) {
-      const float2 v = unpack2(h[i]);
-      sH[(2 * i) * NT + tid] = v.x;
-      sH[(2 * i + 1) * NT + tid] = v.y;
+    for (int j = 0; j < NP; ++j) {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) sH[(j * NS + i) * NT + tid] = h[j][i];
+      sH[(NP * NS + j) * NT + tid] = steps[j];
     }
-    sH[NS * NT + tid] = steps;
     cluster.sync();
-    for (int j = 0; j < part; ++j) {
-      const float* peer = cluster.map_shared_rank(sH, j);
-      const float sum = peer[NS * NT + tid];
+    for (int k = 0; k < part; ++k) {
+      const f32x2* peer = cluster.map_shared_rank(sH, k) + tid;
 #pragma unroll
-      for (int i = 0; i < NS / 2; ++i) {
-        const float2 e = unpack2(mul2(a[i], pack2(sum, sum)));
-        start[i] = fma2(pack2(ex2(e.x), ex2(e.y)), start[i], pack2(peer[(2 * i) * NT + tid], peer[(2 * i + 1) * NT + tid]));
+      for (int j = 0; j < NP; ++j) {
+        const f32x2 sum = peer[(NP * NS + j) * NT];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+          const float2 e = unpack2(mul2(a[j][i], sum));
+          start[j][i] = fma2(pack2(ex2(e.x), ex2(e.y)), start[j][i], peer[(j * NS + i) * NT]);
+        }
       }
     }
     cluster.sync();  // peers have read; the state row may be written now
 #pragma unroll
-    for (int i = 0; i < NS / 2; ++i) h[i] = start[i];
+    for (int j = 0; j < NP; ++j)
+#pragma unroll
+      for (int i = 0; i < NS; ++i) h[j][i] = start[j][i];
     run(b0, b1, true);
     if (part + 1 < q.parts) return;
   } else {
     run(0, sp.len, true);
   }
-  if (on && p.h_out) {
+  if (!p.h_out) return;
 #pragma unroll
-    for (int i = 0; i < NS / 2; ++i) {
-      const float2 v = unpack2(h[i]);
-      p.h_out[hoff + 2 * i] = v.x;
-      p.h_out[hoff + 2 * i + 1] = v.y;
+  for (int j = 0; j < NP; ++j) {
+    const int c = 2 * (ch + j * CBP);
+    float* hp = p.h_out + (row * p.D + c0 + c) * N + lane * NS;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const float2 v = unpack2(h[j][i]);
+      if (c < cn) hp[i] = v.x;
+      if (c + 1 < cn) hp[N + i] = v.y;
     }
   }
 }
@@ -464,12 +587,9 @@ int allow(int bytes, bool big_cluster) {
   return WKVM_OK;
 }
 
-template <typename T, int N>
+template <typename T, int N, int NP, int NS, int NT, int TT>
 int launch_tiles(const ScanArgs& s, cudaStream_t st) {
-  // two states a thread keep two warps on every scheduler at a few thousand
-  // channels of one sequence; 128 states would need two warps per channel
-  constexpr int NS = N == 128 ? 4 : 2, NT = 256;
-  using K = Tile<N, NS, NT>;
+  using K = Tile<T, N, NP, NS, NT, TT>;
   TileArgs q{s, 0, 1, false, false, false};
   const int per_group = s.D / s.G;
   q.cblocks = (per_group + K::CB - 1) / K::CB;
@@ -481,21 +601,21 @@ int launch_tiles(const ScanArgs& s, cudaStream_t st) {
             (!s.z.p || (even(s.z, K::VE) && aligned_to(s.z.p, ax)));
   q.vec_b = even(s.B, K::VB) && even(s.C, K::VB) && aligned_to(s.B.p, ab) && aligned_to(s.C.p, ab);
   q.longest_first = s.seqs.cu && s.seqs.nseq > 1 && s.seqs.nseq <= 256;
-  // split sequences in time when the whole ones would leave most SMs idle:
-  // a split pays twice for the exponentials, so two parts gain nothing
+  // Split sequences in time when whole ones give the SMs too few warps: a
+  // split pays twice for the exponentials, so two parts gain nothing.
   const int64_t tokens = s.seqs.cu ? s.seqs.T / s.seqs.nseq : s.seqs.T;
   int parts = 1;
-  while (parts < 16 && jobs * parts * 2 <= 296 && tokens >= (int64_t)parts * 2 * 2 * kTT) parts *= 2;
+  while (parts < 16 && jobs * parts * 2 <= 2048 && tokens >= (int64_t)parts * 8 * TT) parts *= 2;
   if (parts < 4) parts = 1;
-  if (jobs * parts > INT32_MAX) return WKVM_ERR_SHAPE;
   q.parts = parts;
+  if (jobs * parts > INT32_MAX) return WKVM_ERR_SHAPE;
   if (parts == 1) {
-    constexpr auto kern = scan_tiles_kernel<T, N, NS, NT, false>;
+    constexpr auto kern = scan_tiles_kernel<T, N, NP, NS, NT, TT, false>;
     if (int rc = allow<kern>(K::bytes(false), false)) return rc;
     kern<<<(unsigned)jobs, NT, K::bytes(false), st>>>(q);
     return cudaGetLastError() == cudaSuccess ? WKVM_OK : WKVM_ERR_CUDA;
   }
-  constexpr auto kern = scan_tiles_kernel<T, N, NS, NT, true>;
+  constexpr auto kern = scan_tiles_kernel<T, N, NP, NS, NT, TT, true>;
   if (int rc = allow<kern>(K::bytes(true), true)) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(jobs * parts));
@@ -515,7 +635,8 @@ template <typename T, int N>
 int launch_scan_n(const ScanArgs& a, cudaStream_t st) {
   // a few tokens of every row: the state's traffic decides, so the row kernel
   if (!a.seqs.cu && a.seqs.T <= 8) return launch_rows<T, N>(a, st);
-  return launch_tiles<T, N>(a, st);
+  constexpr int NS = N == 128 ? 8 : 4;
+  return launch_tiles<T, N, 1, NS, 32, 16>(a, st);
 }
 
 template <typename T>

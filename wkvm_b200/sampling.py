@@ -8,6 +8,9 @@ from . import _lib
 from . import ops as _ops
 
 
+MAX_VOCAB = 393216  # a row is held in the shared memory of eight CTAs
+
+
 def _setting(name: str, value, rows: int, dtype: torch.dtype, logits: torch.Tensor):
     """(per-row device tensor or None, scalar) of one sampling setting."""
     if not isinstance(value, torch.Tensor):
@@ -49,7 +52,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     if logits.dtype not in _ops._DTYPES:
         raise ValueError(f"unsupported dtype {logits.dtype}")
     B, V = logits.shape
-    if V < 1 or V >= 1 << 31:
+    if V < 1 or V > MAX_VOCAB:
         raise ValueError(f"a vocabulary of {V} is not supported")
     if u.dim() != 1 or u.shape[0] != B:
         raise ValueError(f"u must be [{B}], not {tuple(u.shape)}")
