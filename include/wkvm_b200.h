@@ -367,7 +367,7 @@ int wkvm_selective_scan_slots(
     int32_t D, int32_t N, int32_t G, int32_t softplus, int32_t dtype,
     int32_t* status, wkvm_stream_t stream);
 
-enum { WKVM_SAMPLE_MAX_VOCAB = 393216 };
+enum { WKVM_SAMPLE_MAX_VOCAB = 1 << 30 };
 
 /* Chooses one token for each of B rows of V logits (row_stride elements
  * apart) from a given uniform number u[b] in [0, 1). With m the row's

@@ -21,14 +21,13 @@
 // moves a mass by V 2^-(s+1) at most, 2^-31 of the largest weight there.
 //
 // All three filters keep a prefix of the descending order, so what is kept is
-// one logit and a bound on the ids that equal it. A cluster of CTAs holds a
-// row in shared memory (logits are read from HBM once) and finds that bound
-// by histograms of counts (top-k) or masses (top-p) over the logits above a
-// lower bound, then finishes on a sorted list of at most kCap candidates in
-// one CTA. Only a larger set is narrowed by further histograms and drawn from
-// by a pass over the whole row. 65,536 logits cost 2.1e6 fp64 operations in
-// exponentials, which with the passes over shared memory and the cluster's
-// barriers bound it; HBM does not.
+// one logit and a bound on the ids that equal it. A row's CTAs (one when there
+// are many rows, a cluster when there are few) find that bound by histograms
+// of counts (top-k) or masses (top-p) over the logits above a lower bound,
+// then finish on a sorted list of at most kCap candidates in one CTA. Only a
+// larger set is narrowed by further histograms and drawn from by a pass over
+// the whole row. HBM is read once: later passes find short slices in shared
+// memory and long ones in L2 (148 rows of 65,536 fp32 logits are 39 MB).
 #include <cooperative_groups.h>
 
 #include <atomic>
@@ -53,6 +52,7 @@ struct SampleArgs {
   float* logprob;
   int32_t V;
   int32_t slice;  // logits of one CTA, a multiple of kNT
+  int32_t ctas;   // of a row
   double shift;   // 2^(52-s): adding it leaves a weight's units in the low bits
   bool vec;       // rows start on 16 bytes
 };
@@ -61,6 +61,7 @@ constexpr int kNT = 512, kWarps = kNT / 32;
 constexpr int kBins = 1024;
 constexpr int kCap = 1024;        // candidates one CTA sorts
 constexpr int kMaxCtas = 8;       // CTAs of a row (portable cluster size)
+constexpr int kSmemSlice = 16384; // logits of a slice kept in shared memory (two CTAs an SM)
 
 // Ascending unsigned order of floats; -inf is 0 and never kept (NaN and -0
 // are gone by then).
@@ -103,10 +104,14 @@ struct Found {          // what a level of a selection found, the same in every 
 // Shared memory of a CTA ahead of its slice of logits. Fields named peer_* are
 // written by the other CTAs of the cluster, [rank] by rank.
 struct Shared {
-  uint32_t cnt[kBins];              // histogram: counts
-  uint32_t mass_lo[kBins], mass_hi[kBins];  // and masses
-  u64 list[kCap];                   // candidates: ~key << 32 | id, ascending = the descending order
-  u64 weight[kCap];
+  union {
+    struct {                          // histogram: counts, and masses in two words
+      uint32_t cnt[kBins], mass_lo[kBins], mass_hi[kBins];
+    };
+    struct {                          // then candidates: ~key << 32 | id, ascending = the descending order
+      u64 list[kCap], weight[kCap];
+    };
+  };
   u64 warp_sum[kWarps];
   uint32_t warp_u32[3][kWarps];
   uint32_t peer_max[kMaxCtas], peer_warp[kMaxCtas], peer_thread[kMaxCtas];
@@ -117,12 +122,18 @@ struct Shared {
   uint32_t tau;                     // the last kept key
   int32_t limit;                    // ids below it are kept among its equals
   int32_t first;                    // greedy
+  int32_t owner;                    // the warp whose block holds the drawn token
 };
 
+template <typename T, bool SMEM>
 struct Row {
+  static constexpr int kVec = 16 / sizeof(T);
   Shared* s;
-  const float* vals;
+  const float* vals;  // SMEM: the slice, NaN and -0 replaced
+  const T* row;       // the slice in global memory
+  bool vec;           // it starts on 16 bytes
   int rank, ctas, tid, lane, warp, slice, base;  // base: the slice's first id
+  int n;              // logits of the slice that exist
   double m, c;       // maximum; log2(e) / temperature
   double shift;      // of units(), a power of two >= 1
   uint32_t mkey;
@@ -141,8 +152,41 @@ struct Row {
   __device__ u64 mass(float l) const { return units(weight(l)); }
   __device__ bool kept(uint32_t k, int id) const { return k > tau || (k == tau && id < limit); }
 
-  template <typename T>
-  __device__ T warp_add(T x) const {
+  // NaN counts as -inf, -0 as 0
+  __device__ static float clean(float v) { return v > -INFINITY ? v + 0.f : -INFINITY; }
+  __device__ float at(int i) const {
+    if constexpr (SMEM) return vals[i];
+    return i < n ? clean(to_f32(row[i])) : -INFINITY;
+  }
+  // f(logit, index) for the logits [i0, i1) that exist, dealt to `nt` threads
+  // of which this is thread t; i0 is a multiple of kVec.
+  template <typename F>
+  __device__ __forceinline__ void each(int i0, int i1, int t, int nt, F f) const {
+    if (i1 > n) i1 = n;
+    if constexpr (SMEM) {
+      for (int i = i0 + t; i < i1; i += nt) f(vals[i], i);
+    } else {
+      const int whole = vec && i1 > i0 ? i0 + (i1 - i0) / kVec * kVec : i0;
+      // two vectors in flight a thread
+      for (int i = i0 + t * kVec; i < whole; i += 2 * nt * kVec) {
+        const int i2 = i + nt * kVec;
+        const uint4 a = *reinterpret_cast<const uint4*>(row + i);
+        const uint4 b = i2 < whole ? *reinterpret_cast<const uint4*>(row + i2) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) f(clean(to_f32(reinterpret_cast<const T*>(&a)[j])), i + j);
+        if (i2 < whole) {
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) f(clean(to_f32(reinterpret_cast<const T*>(&b)[j])), i2 + j);
+        }
+      }
+      for (int i = whole + t; i < i1; i += nt) f(clean(to_f32(row[i])), i);
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const { each(0, slice, tid, kNT, f); }
+
+  template <typename X>
+  __device__ X warp_add(X x) const {
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
     return x;
@@ -157,8 +201,10 @@ struct Row {
     for (int i = 0; i < kWarps; ++i) t += s->warp_sum[i];
     return t;
   }
-  __device__ Shared* peer(int r) const { return cg::this_cluster().map_shared_rank(s, r); }
-  __device__ static void sync() { cg::this_cluster().sync(); }  // the row's CTAs
+  __device__ Shared* peer(int r) const { return ctas == 1 ? s : cg::this_cluster().map_shared_rank(s, r); }
+  __device__ void sync() const {  // the row's CTAs
+    if (ctas == 1) __syncthreads(); else cg::this_cluster().sync();
+  }
 };
 
 // A level's bins: keys [lo, hi] into kBins bins, the largest first. Linear in
@@ -184,8 +230,8 @@ struct Bins {
 // the first bin at which above + the running count (or mass) reaches the goal.
 // `rest`: mass of what is kept below b.lo joins the total, and the goal is
 // share times that total (first level of top-p). Two cluster barriers.
-template <bool MASS>
-__device__ void level(Row& r, const Bins& b, uint32_t above, u64 mass_above, double goal, bool rest,
+template <bool MASS, typename R>
+__device__ void level(R& r, const Bins& b, uint32_t above, u64 mass_above, double goal, bool rest,
                       double share, u64* total) {
   Shared* s = r.s;
   for (int i = r.tid; i < kBins; i += kNT) {
@@ -194,14 +240,13 @@ __device__ void level(Row& r, const Bins& b, uint32_t above, u64 mass_above, dou
   }
   __syncthreads();
   u64 all = 0;
-  for (int i = r.tid; i < r.slice; i += kNT) {
-    const float l = r.vals[i];
+  r.each([&](float l, int i) {
     const uint32_t k = key_of(l);
-    if (k > b.hi || (k < b.lo && !rest) || !r.kept(k, r.base + i)) continue;
+    if (k > b.hi || (k < b.lo && !rest) || !r.kept(k, r.base + i)) return;
     u64 w = 0;
     if (MASS) w = r.mass(l);
     if (MASS && rest) all += w;
-    if (k < b.lo) continue;
+    if (k < b.lo) return;
     const int bin = b(l, k);
     atomicAdd(&s->cnt[bin], 1u);
     if (MASS) {
@@ -209,7 +254,7 @@ __device__ void level(Row& r, const Bins& b, uint32_t above, u64 mass_above, dou
       const uint32_t hi = (uint32_t)(w >> 32) + (old + lo < old);
       if (hi) atomicAdd(&s->mass_hi[bin], hi);
     }
-  }
+  });
   if (MASS && rest) {
     all = r.block_add(all);
     if (r.tid < r.ctas) r.peer(r.tid)->peer_total[r.rank] = all;
@@ -279,26 +324,27 @@ __device__ void level(Row& r, const Bins& b, uint32_t above, u64 mass_above, dou
 }
 
 // Kept candidates whose bin is `bin` (or above it too) go to the first CTA's list.
-__device__ void gather(Row& r, const Bins& b, int bin, bool above_too) {
+template <typename R>
+__device__ void gather(R& r, const Bins& b, int bin, bool above_too) {
   Shared* first = r.peer(0);
-  for (int i = r.tid; i < r.slice; i += kNT) {
-    const float l = r.vals[i];
+  r.each([&](float l, int i) {
     const uint32_t k = key_of(l);
-    if (k < b.lo || !r.kept(k, r.base + i)) continue;
+    if (k < b.lo || !r.kept(k, r.base + i)) return;
     if (k > b.hi) {
-      if (!above_too) continue;
+      if (!above_too) return;
     } else {
       const int at = b(l, k);
-      if (above_too ? at > bin : at != bin) continue;
+      if (above_too ? at > bin : at != bin) return;
     }
     const uint32_t slot = atomicAdd(&first->n_list, 1u);
     if (slot < kCap) first->list[slot] = ((u64)~k << 32) | (uint32_t)(r.base + i);
-  }
+  });
   r.sync();
 }
 
 // Sorts the first n entries of the list ascending (one CTA, n <= kCap).
-__device__ void sort_list(Row& r, int n) {
+template <typename R>
+__device__ void sort_list(R& r, int n) {
   Shared* s = r.s;
   int size = 2;
   while (size < n) size *= 2;
@@ -319,7 +365,8 @@ __device__ void sort_list(Row& r, int n) {
 }
 
 // Inclusive sums of weight[0, n) in place (one CTA, two neighbours a thread).
-__device__ void scan_weights(Row& r, int n) {
+template <typename R>
+__device__ void scan_weights(R& r, int n) {
   Shared* s = r.s;
   const int i = 2 * r.tid;
   const u64 a = i < n ? s->weight[i] : 0, b = i + 1 < n ? s->weight[i + 1] : 0;
@@ -342,7 +389,8 @@ __device__ __forceinline__ uint32_t list_key(u64 e) { return ~(uint32_t)(e >> 32
 
 // The row's end on the list: n candidates, of which the first k are in play.
 // total: the mass top-p takes its share of (0: of these k).
-__device__ void finish_list(Row& r, int n, int k, double tp, double mp, double u, u64 total,
+template <typename R>
+__device__ void finish_list(R& r, int n, int k, double tp, double mp, double u, u64 total,
                             int64_t* token, float* logprob) {
   Shared* s = r.s;
   sort_list(r, n);
@@ -387,11 +435,12 @@ __device__ void finish_list(Row& r, int n, int k, double tp, double mp, double u
 }
 
 // Keeps, of the kept candidates that equal `key`, the `want` lowest ids.
-__device__ void limit_ties(Row& r, uint32_t key, uint32_t want) {
+template <typename R>
+__device__ void limit_ties(R& r, uint32_t key, uint32_t want) {
   Shared* s = r.s;
   const int per = r.slice / kWarps, i0 = r.warp * per;
   uint32_t c = 0;
-  for (int i = i0 + r.lane; i < i0 + per; i += 32) c += key_of(r.vals[i]) == key && r.kept(key, r.base + i);
+  r.each(i0, i0 + per, r.lane, 32, [&](float l, int i) { c += key_of(l) == key && r.kept(key, r.base + i); });
   c = r.warp_add(c);
   __syncthreads();
   if (r.lane == 0) s->warp_u32[0][r.warp] = c;
@@ -407,7 +456,7 @@ __device__ void limit_ties(Row& r, uint32_t key, uint32_t want) {
   for (int w = 0; w < r.warp; ++w) before += s->warp_u32[0][w];
   if (before < want && before + s->warp_u32[0][r.warp] >= want) {  // one warp of the cluster
     for (int i = i0; i < i0 + per; i += 32) {
-      const bool is = key_of(r.vals[i + r.lane]) == key && r.kept(key, r.base + i + r.lane);
+      const bool is = key_of(r.at(i + r.lane)) == key && r.kept(key, r.base + i + r.lane);
       const uint32_t b = __ballot_sync(0xffffffffu, is);
       if (before + __popc(b) < want) {
         before += __popc(b);
@@ -427,8 +476,8 @@ __device__ void limit_ties(Row& r, uint32_t key, uint32_t want) {
 // Narrows what is kept to the first candidates in descending order whose
 // count reaches `goal` (or whose mass reaches tp of the mass of all kept).
 // Returns true when the row was finished on the list.
-template <bool MASS>
-__device__ bool select(Row& r, uint32_t lo, double goal, int k, double tp, double mp, double u,
+template <bool MASS, typename R>
+__device__ bool select(R& r, uint32_t lo, double goal, int k, double tp, double mp, double u,
                        int64_t* token, float* logprob) {
   Shared* s = r.s;
   Bins b(lo, r.mkey);
@@ -475,13 +524,12 @@ __device__ bool select(Row& r, uint32_t lo, double goal, int k, double tp, doubl
     }
     // too many: their smallest and largest key bound the next level
     uint32_t kl = 0xffffffffu, kh = 0;
-    for (int i = r.tid; i < r.slice; i += kNT) {
-      const float l = r.vals[i];
+    r.each([&](float l, int i) {
       const uint32_t q = key_of(l);
-      if (q < b.lo || q > b.hi || !r.kept(q, r.base + i) || b(l, q) != f.bin) continue;
+      if (q < b.lo || q > b.hi || !r.kept(q, r.base + i) || b(l, q) != f.bin) return;
       kl = min(kl, q);
       kh = max(kh, q);
-    }
+    });
     kl = __reduce_min_sync(0xffffffffu, kl);
     kh = __reduce_max_sync(0xffffffffu, kh);
     __syncthreads();
@@ -520,15 +568,17 @@ __device__ bool select(Row& r, uint32_t lo, double goal, int k, double tp, doubl
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kNT) sample_kernel(SampleArgs p) {
+template <typename T, bool SMEM>
+__global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
   extern __shared__ __align__(16) uint8_t smem[];
-  Row r;
+  using R = Row<T, SMEM>;
+  constexpr int kVec = R::kVec;
+  R r;
   Shared* s = r.s = reinterpret_cast<Shared*>(smem);
   float* vals = reinterpret_cast<float*>(smem + sizeof(Shared));
   r.vals = vals;
-  r.rank = (int)cg::this_cluster().block_rank();
-  r.ctas = (int)cg::this_cluster().num_blocks();
+  r.ctas = p.ctas;
+  r.rank = (int)(blockIdx.x % p.ctas);
   r.tid = threadIdx.x;
   r.lane = r.tid & 31;
   r.warp = r.tid >> 5;
@@ -536,26 +586,39 @@ __global__ void __launch_bounds__(kNT) sample_kernel(SampleArgs p) {
   r.base = r.rank * p.slice;
   r.tau = 0;  // key 0 is never kept
   r.limit = 0;
-  const int b = blockIdx.x / r.ctas;
-  const T* row = static_cast<const T*>(p.logits) + b * p.row_stride + r.base;
-  const int n = min(p.slice, p.V - r.base);  // may be <= 0
+  r.vec = p.vec;
+  const int b = blockIdx.x / p.ctas;
+  r.row = static_cast<const T*>(p.logits) + b * p.row_stride + r.base;
+  r.n = max(0, min(p.slice, p.V - r.base));
 
-  // ---- the slice into shared memory, and its maximum
+  // ---- the slice's maximum (and the slice into shared memory), four vectors
+  //      in flight a thread
   uint32_t mine = 0;
   auto put = [&](int i, float v) {
-    v = v > -INFINITY ? v + 0.f : -INFINITY;  // NaN counts as -inf, -0 as 0
-    vals[i] = v;
+    v = R::clean(v);
+    if constexpr (SMEM) vals[i] = v;
     mine = max(mine, key_of(v));
   };
-  constexpr int kVec = 16 / sizeof(T);
-  const int whole = p.vec ? max(n, 0) / kVec * kVec : 0;
-  for (int i = r.tid * kVec; i < whole; i += kNT * kVec) {
-    const uint4 q = *reinterpret_cast<const uint4*>(row + i);
-    const T* e = reinterpret_cast<const T*>(&q);
+  constexpr int kFly = 4;
+  const int whole = p.vec ? r.n / kVec * kVec : 0;
+  for (int i0 = r.tid * kVec; i0 < whole; i0 += kFly * kNT * kVec) {
+    uint4 q[kFly];
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) put(i + j, to_f32(e[j]));
+    for (int f = 0; f < kFly; ++f) {
+      const int i = i0 + f * kNT * kVec;
+      if (i < whole) q[f] = *reinterpret_cast<const uint4*>(r.row + i);
+    }
+#pragma unroll
+    for (int f = 0; f < kFly; ++f) {
+      const int i = i0 + f * kNT * kVec;
+      if (i >= whole) break;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) put(i + j, to_f32(reinterpret_cast<const T*>(&q[f])[j]));
+    }
   }
-  for (int i = whole + r.tid; i < p.slice; i += kNT) put(i, i < n ? to_f32(row[i]) : -INFINITY);
+  for (int i = whole + r.tid; i < r.n; i += kNT) put(i, to_f32(r.row[i]));
+  if constexpr (SMEM)
+    for (int i = r.n + r.tid; i < p.slice; i += kNT) vals[i] = -INFINITY;
 
   const double u = p.u[b];
   float temp = p.temperature ? p.temperature[b] : p.temperature0;
@@ -572,17 +635,17 @@ __global__ void __launch_bounds__(kNT) sample_kernel(SampleArgs p) {
   }
   if (r.tid == 0) s->first = INT32_MAX;
   __syncthreads();
-  if (r.tid < r.ctas) {
-    uint32_t mx = 0, mw = 0xffffffffu, mt = 0xffffffffu;
-    for (int w = 0; w < kWarps; ++w) {
-      mx = max(mx, s->warp_u32[0][w]);
-      mw = min(mw, s->warp_u32[0][w]);
-      mt = min(mt, s->warp_u32[1][w]);
+  if (r.warp == 0) {
+    const bool have = r.lane < kWarps;
+    const uint32_t mx = __reduce_max_sync(0xffffffffu, have ? s->warp_u32[0][r.lane] : 0u);
+    const uint32_t mw = __reduce_min_sync(0xffffffffu, have ? s->warp_u32[0][r.lane] : 0xffffffffu);
+    const uint32_t mt = __reduce_min_sync(0xffffffffu, have ? s->warp_u32[1][r.lane] : 0xffffffffu);
+    if (r.lane < r.ctas) {
+      Shared* o = r.peer(r.lane);
+      o->peer_max[r.rank] = mx;
+      o->peer_warp[r.rank] = mw;
+      o->peer_thread[r.rank] = mt;
     }
-    Shared* o = r.peer(r.tid);
-    o->peer_max[r.rank] = mx;
-    o->peer_warp[r.rank] = mw;
-    o->peer_thread[r.rank] = mt;
   }
   r.sync();
   uint32_t least_w = 0xffffffffu, least_t = 0xffffffffu;
@@ -605,11 +668,9 @@ __global__ void __launch_bounds__(kNT) sample_kernel(SampleArgs p) {
 
   if (k == 1) {  // the lowest id of the largest logit
     int at = INT32_MAX;
-    for (int i = r.tid; i < p.slice; i += kNT)
-      if (key_of(vals[i]) == r.mkey) {
-        at = i + r.base;
-        break;
-      }
+    r.each([&](float l, int i) {
+      if (key_of(l) == r.mkey) at = min(at, i + r.base);
+    });
     at = __reduce_min_sync(0xffffffffu, at);
     if (r.lane == 0 && at != INT32_MAX) atomicMin(&r.peer(0)->first, at);
     r.sync();
@@ -638,20 +699,21 @@ __global__ void __launch_bounds__(kNT) sample_kernel(SampleArgs p) {
   const int per = p.slice / kWarps, i0 = r.warp * per;
   // logits this low have w < mp for certain
   const float low = mp > 0.0 ? (float)(r.m + log2(mp) / r.c * 1.0001 - fabs(r.m) * 3e-7) : -INFINITY;
-  auto share = [&](int i, double* w) -> u64 {
-    const float l = vals[i];
+  auto share = [&](float l, int i, double* w) -> u64 {
     const uint32_t q = key_of(l);
-    if (q != r.mkey && (l < low || !r.kept(q, r.base + i))) return 0;
-    if (q == r.mkey && !r.kept(q, r.base + i)) return 0;
+    if ((q != r.mkey && l < low) || !r.kept(q, r.base + i)) return 0;
     *w = r.weight(l);
     return *w >= mp || q == r.mkey ? r.units(*w) : 0;
   };
   u64 sum = 0;
-  double w;
-  for (int i = i0 + r.lane; i < i0 + per; i += 32) sum += share(i, &w);
+  r.each(i0, i0 + per, r.lane, 32, [&](float l, int i) {
+    double w;
+    sum += share(l, i, &w);
+  });
   sum = r.warp_add(sum);
   __syncthreads();
   if (r.lane == 0) s->warp_sum[r.warp] = sum;
+  if (r.tid == 0) s->owner = -1;
   __syncthreads();
   if (r.tid < r.ctas) {
     u64 t = 0;
@@ -667,19 +729,39 @@ __global__ void __launch_bounds__(kNT) sample_kernel(SampleArgs p) {
   for (int i = 0; i < r.warp; ++i) before += s->warp_sum[i];
   double goal = u * (double)z;
   if (!(goal < (double)z)) goal = (double)(z - 1);
-  // the one warp in whose block the running mass passes the goal
-  if (sum == 0 || (double)before > goal || !((double)(before + sum) > goal)) return;
-  for (int i = i0; i < i0 + per; i += 32) {
-    w = 0.0;
-    const u64 own = share(i + r.lane, &w);
+  // the one block in which the running mass passes the goal is split again
+  // over the warps of its CTA
+  auto holds = [&](u64 from, u64 mass) { return mass && !((double)from > goal) && (double)(from + mass) > goal; };
+  if (holds(before, sum) && r.lane == 0) {
+    s->owner = r.warp;
+    s->peer_total[0] = before;
+  }
+  __syncthreads();
+  if (s->owner < 0) return;
+  const int part = (per / kWarps + 31) / 32 * 32, j0 = s->owner * per, j1 = j0 + per;
+  const int p0 = min(j0 + r.warp * part, j1), p1 = min(p0 + part, j1);
+  before = s->peer_total[0];
+  sum = 0;
+  for (int i = p0 + r.lane; i < p1; i += 32) {
+    double w;
+    sum += share(r.at(i), i, &w);
+  }
+  sum = r.warp_add(sum);
+  __syncthreads();
+  if (r.lane == 0) s->warp_sum[r.warp] = sum;
+  __syncthreads();
+  for (int i = 0; i < r.warp; ++i) before += s->warp_sum[i];
+  if (!holds(before, sum)) return;
+  for (int i = p0; i < p1; i += 32) {
+    double w = 0.0;
+    const u64 own = share(r.at(i + r.lane), i + r.lane, &w);  // blocks are whole warps wide
     u64 x = own;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
       const u64 up = __shfl_up_sync(0xffffffffu, x, off);
       if (r.lane >= off) x += up;
     }
-    const bool hit = own && (double)(before + x) > goal;
-    const uint32_t any = __ballot_sync(0xffffffffu, hit);
+    const uint32_t any = __ballot_sync(0xffffffffu, own && (double)(before + x) > goal);
     if (any) {
       if (r.lane == __ffs(any) - 1) {
         p.token[b] = r.base + i + r.lane;
@@ -691,28 +773,36 @@ __global__ void __launch_bounds__(kNT) sample_kernel(SampleArgs p) {
   }
 }
 
-template <typename T>
-int launch(const SampleArgs& a, int B, int ctas, cudaStream_t st) {
-  const int bytes = (int)sizeof(Shared) + a.slice * 4;
-  static std::atomic<uint64_t> done{0};  // a bit per device: the shared-memory limit is raised
-  int dev = 0;
-  WKVM_CUDA_TRY(cudaGetDevice(&dev));
-  if (dev >= 64 || !(done.load(std::memory_order_acquire) >> dev & 1)) {
-    WKVM_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 << 10));
-    if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
+template <typename T, bool SMEM>
+int launch_on(const SampleArgs& a, int B, cudaStream_t st) {
+  const int bytes = (int)sizeof(Shared) + (SMEM ? a.slice * 4 : 0);
+  if (SMEM) {
+    static std::atomic<uint64_t> done{0};  // a bit per device: the shared-memory limit is raised
+    int dev = 0;
+    WKVM_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev >= 64 || !(done.load(std::memory_order_acquire) >> dev & 1)) {
+      WKVM_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T, SMEM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)sizeof(Shared) + kSmemSlice * 4));
+      if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
+    }
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((int64_t)B * ctas));
+  cfg.gridDim = dim3((unsigned)((int64_t)B * a.ctas));
   cfg.blockDim = dim3(kNT);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)ctas;
+  attr[0].val.clusterDim.x = (unsigned)a.ctas;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, sample_kernel<T>, a) == cudaSuccess ? WKVM_OK : WKVM_ERR_CUDA;
+  cfg.numAttrs = a.ctas > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, sample_kernel<T, SMEM>, a) == cudaSuccess ? WKVM_OK : WKVM_ERR_CUDA;
+}
+
+template <typename T>
+int launch(const SampleArgs& a, int B, cudaStream_t st) {
+  return a.slice <= kSmemSlice ? launch_on<T, true>(a, B, st) : launch_on<T, false>(a, B, st);
 }
 
 }  // namespace
@@ -731,9 +821,10 @@ extern "C" int wkvm_sample_tokens(const void* logits, int64_t row_stride, const 
   if (V > WKVM_SAMPLE_MAX_VOCAB) return WKVM_ERR_SHAPE;
   if (B == 0) return WKVM_OK;
   if (!logits || !u || !tokens || !logprobs) return WKVM_ERR_INVALID_ARG;
-  // about 8,192 logits a CTA: sixteen a thread
+  // Rows alone fill the 148 SMs from 128 on; fewer are split over a cluster
+  // as long as a CTA keeps two logits a thread.
   int ctas = 1;
-  while (ctas < wkvm::kMaxCtas && V > ctas * 8192) ctas *= 2;
+  while (ctas < wkvm::kMaxCtas && (int64_t)B * ctas < 128 && V >= ctas * 2048) ctas *= 2;
   if ((int64_t)B * ctas > INT32_MAX) return WKVM_ERR_SHAPE;
   const int64_t es = dtype == WKVM_DTYPE_F32 ? 4 : 2;
   const int slice = ((V + ctas - 1) / ctas + wkvm::kNT - 1) / wkvm::kNT * wkvm::kNT;
@@ -741,11 +832,11 @@ extern "C" int wkvm_sample_tokens(const void* logits, int64_t row_stride, const 
   double shift = 1.0;  // s = min(52, 62 - ceil(log2 V))
   for (int64_t v = 1 << 10; v < V; v *= 2) shift *= 2.0;
   wkvm::SampleArgs a{logits, row_stride, u, temperature, top_p, min_p, top_k, temperature0, top_p0,
-                     min_p0, top_k0, tokens, logprobs, V, slice, shift, vec};
+                     min_p0, top_k0, tokens, logprobs, V, slice, ctas, shift, vec};
   cudaStream_t st = (cudaStream_t)stream;
   switch (dtype) {
-    case WKVM_DTYPE_F32: return wkvm::launch<float>(a, B, ctas, st);
-    case WKVM_DTYPE_BF16: return wkvm::launch<__nv_bfloat16>(a, B, ctas, st);
-    default: return wkvm::launch<__half>(a, B, ctas, st);
+    case WKVM_DTYPE_F32: return wkvm::launch<float>(a, B, st);
+    case WKVM_DTYPE_BF16: return wkvm::launch<__nv_bfloat16>(a, B, st);
+    default: return wkvm::launch<__half>(a, B, st);
   }
 }

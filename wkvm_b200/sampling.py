@@ -8,7 +8,7 @@ from . import _lib
 from . import ops as _ops
 
 
-MAX_VOCAB = 393216  # a row is held in the shared memory of eight CTAs
+MAX_VOCAB = 1 << 30  # WKVM_SAMPLE_MAX_VOCAB
 
 
 def _setting(name: str, value, rows: int, dtype: torch.dtype, logits: torch.Tensor):
