@@ -60,6 +60,7 @@ struct SampleArgs {
 constexpr int kNT = 512, kWarps = kNT / 32;
 constexpr int kBins = 1024;
 constexpr int kCap = 1024;        // candidates one CTA sorts
+constexpr int kGroups = 6;        // sets of 32, 16, .. 1 threads
 constexpr int kMaxCtas = 8;       // CTAs of a row (portable cluster size)
 constexpr int kSmemSlice = 16384; // logits of a slice kept in shared memory (two CTAs an SM)
 
@@ -74,25 +75,29 @@ __device__ __forceinline__ float value_of(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
 
-// 2^t for -64 <= t <= 0: the power series of e^(f ln 2), |f| <= 1/2, to degree
-// 10 (truncation 2.2e-13), times 2^n through the exponent.
-__device__ __forceinline__ double exp2_neg(double t) {
-  const double magic = 6755399441055744.0;  // 1.5 * 2^52: rounds to an integer
-  const double r = t + magic;
-  const int n = __double2loint(r);
-  const double f = t - (r - magic);
-  double p = 7.0549116208011233e-09;
-  p = fma(p, f, 1.0178086009239699e-07);
-  p = fma(p, f, 1.3215486790144309e-06);
-  p = fma(p, f, 1.5252733804059841e-05);
-  p = fma(p, f, 1.5403530393381609e-04);
-  p = fma(p, f, 1.3333558146428443e-03);
-  p = fma(p, f, 9.6181291076284772e-03);
-  p = fma(p, f, 5.5504108664821580e-02);
-  p = fma(p, f, 2.4022650695910072e-01);
-  p = fma(p, f, 6.9314718055994531e-01);
-  p = fma(p, f, 1.0);
-  return __hiloint2double(__double2hiint(p) + (n << 20), __double2loint(p));
+// fp32 to fp64 by the bits: the conversion instruction has a quarter of the
+// fp64 pipe's rate. Zero and subnormals become 2^-127 or so, infinities 2^128;
+// both are as good here.
+__device__ __forceinline__ double widen(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));
+}
+
+// 2^t for -1000 < t <= 0, to 1e-13: with k = t rounded to 1/64 and r the rest,
+// 2^(k >> 6) times table[k & 63] = 2^((k & 63) / 64) times 1 + r p(r), the
+// power series of e^(r ln 2) to degree 4 (|r ln 2| < 0.0055).
+__device__ __forceinline__ double exp2_neg(double t, const double* table) {
+  const double magic = 105553116266496.0;  // 1.5 * 2^46: rounds to 1/64
+  const double u = t + magic;
+  const int k = __double2loint(u);
+  const double r = t - (u - magic);
+  double p = 0.009618129107628477;
+  p = fma(p, r, 0.05550410866482158);
+  p = fma(p, r, 0.24022650695910072);
+  p = fma(p, r, 0.6931471805599453);
+  const double e = table[k & 63];
+  const double w = fma(e, r * p, e);
+  return __hiloint2double(__double2hiint(w) + ((k >> 6) << 20), __double2loint(w));
 }
 
 struct Found {          // what a level of a selection found, the same in every CTA
@@ -103,7 +108,7 @@ struct Found {          // what a level of a selection found, the same in every 
 
 // Shared memory of a CTA ahead of its slice of logits. Fields named peer_* are
 // written by the other CTAs of the cluster, [rank] by rank.
-struct Shared {
+struct alignas(16) Shared {
   union {
     struct {                          // histogram: counts, and masses in two words
       uint32_t cnt[kBins], mass_lo[kBins], mass_hi[kBins];
@@ -112,9 +117,10 @@ struct Shared {
       u64 list[kCap], weight[kCap];
     };
   };
+  double exp2_table[64];            // 2^(i / 64)
   u64 warp_sum[kWarps];
-  uint32_t warp_u32[3][kWarps];
-  uint32_t peer_max[kMaxCtas], peer_warp[kMaxCtas], peer_thread[kMaxCtas];
+  uint32_t warp_u32[1 + kGroups][kWarps];
+  uint32_t peer_max[kMaxCtas], peer_least[kGroups][kMaxCtas];
   uint32_t peer_lo[kMaxCtas], peer_hi[kMaxCtas], peer_cnt[kMaxCtas];
   u64 peer_mass[kMaxCtas], peer_total[kMaxCtas];
   Found found;
@@ -124,6 +130,8 @@ struct Shared {
   int32_t first;                    // greedy
   int32_t owner;                    // the warp whose block holds the drawn token
 };
+
+static_assert(sizeof(Shared) % 16 == 0, "the slice behind it is read 16 bytes at a time");
 
 template <typename T, bool SMEM>
 struct Row {
@@ -140,10 +148,32 @@ struct Row {
   uint32_t tau;      // kept: key > tau, or key == tau and id < limit
   int32_t limit;
 
-  __device__ double weight(float l) const {
-    const double t = ((double)l - m) * c;
-    if (__float_as_uint(l) == __float_as_uint((float)m)) return 1.0;
-    return t > -54.0 ? exp2_neg(t) : 0.0;  // less than half a unit (NaN: a maximum of inf)
+  // Four at once: a weight is a chain of some twenty dependent fp64
+  // operations, and only other chains fill its latency.
+  template <int W>
+  __device__ __forceinline__ void weights(const float (&l)[W], double (&w)[W]) const {
+    double t[W];
+    bool in[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      t[j] = (widen(l[j]) - m) * c;
+      // below 2^-54 is less than half a unit: by the exponent and top mantissa
+      // bits, t > -54 (NaN and -inf, of a maximum of inf, are not)
+      in[j] = (uint32_t)__double2hiint(t[j]) < 0xc04b0000u;
+    }
+#pragma unroll
+    for (int j = 0; j < W; ++j) w[j] = exp2_neg(in[j] ? t[j] : -54.0, s->exp2_table);
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      w[j] = in[j] ? w[j] : 0.0;
+      w[j] = l[j] == (float)m ? 1.0 : w[j];
+    }
+  }
+  __device__ __forceinline__ double weight(float l) const {
+    const float a[1] = {l};
+    double w[1];
+    weights<1>(a, w);
+    return w[0];
   }
   __device__ u64 units(double w) const {
     return (u64)(__double_as_longlong(w + shift) - __double_as_longlong(shift));
@@ -158,28 +188,39 @@ struct Row {
     if constexpr (SMEM) return vals[i];
     return i < n ? clean(to_f32(row[i])) : -INFINITY;
   }
-  // f(logit, index) for the logits [i0, i1) that exist, dealt to `nt` threads
-  // of which this is thread t; i0 is a multiple of kVec.
+  // f(logits, i) for the logits [i0, i1) four at a time, i the first one's
+  // index, dealt to `nt` threads of which this is thread t. Past the slice's
+  // end they read as -inf. i0 and i1 are multiples of 8.
   template <typename F>
   __device__ __forceinline__ void each(int i0, int i1, int t, int nt, F f) const {
-    if (i1 > n) i1 = n;
     if constexpr (SMEM) {
-      for (int i = i0 + t; i < i1; i += nt) f(vals[i], i);
+      for (int i = i0 + t * 4; i < i1; i += nt * 4) {
+        const float4 v = *reinterpret_cast<const float4*>(vals + i);
+        const float l[4] = {v.x, v.y, v.z, v.w};
+        f(l, i);
+      }
     } else {
-      const int whole = vec && i1 > i0 ? i0 + (i1 - i0) / kVec * kVec : i0;
-      // two vectors in flight a thread
-      for (int i = i0 + t * kVec; i < whole; i += 2 * nt * kVec) {
-        const int i2 = i + nt * kVec;
-        const uint4 a = *reinterpret_cast<const uint4*>(row + i);
-        const uint4 b = i2 < whole ? *reinterpret_cast<const uint4*>(row + i2) : make_uint4(0, 0, 0, 0);
+      const int whole = vec ? min(i1, max(i0, n / kVec * kVec)) : i0;
+      uint4 next = make_uint4(0, 0, 0, 0);
+      int i = i0 + t * kVec;
+      if (i < whole) next = *reinterpret_cast<const uint4*>(row + i);
+      for (; i < whole; i += nt * kVec) {
+        const uint4 q = next;
+        if (i + nt * kVec < whole) next = *reinterpret_cast<const uint4*>(row + i + nt * kVec);
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) f(clean(to_f32(reinterpret_cast<const T*>(&a)[j])), i + j);
-        if (i2 < whole) {
+        for (int h = 0; h < kVec; h += 4) {
+          float l[4];
 #pragma unroll
-          for (int j = 0; j < kVec; ++j) f(clean(to_f32(reinterpret_cast<const T*>(&b)[j])), i2 + j);
+          for (int j = 0; j < 4; ++j) l[j] = clean(to_f32(reinterpret_cast<const T*>(&q)[h + j]));
+          f(l, i + h);
         }
       }
-      for (int i = whole + t; i < i1; i += nt) f(clean(to_f32(row[i])), i);
+      for (int i = whole + t * 4; i < min(i1, n); i += nt * 4) {
+        float l[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) l[j] = at(i + j);
+        f(l, i);
+      }
     }
   }
   template <typename F>
@@ -240,19 +281,32 @@ __device__ void level(R& r, const Bins& b, uint32_t above, u64 mass_above, doubl
   }
   __syncthreads();
   u64 all = 0;
-  r.each([&](float l, int i) {
-    const uint32_t k = key_of(l);
-    if (k > b.hi || (k < b.lo && !rest) || !r.kept(k, r.base + i)) return;
-    u64 w = 0;
-    if (MASS) w = r.mass(l);
-    if (MASS && rest) all += w;
-    if (k < b.lo) return;
-    const int bin = b(l, k);
-    atomicAdd(&s->cnt[bin], 1u);
-    if (MASS) {
-      const uint32_t lo = (uint32_t)w, old = atomicAdd(&s->mass_lo[bin], lo);
-      const uint32_t hi = (uint32_t)(w >> 32) + (old + lo < old);
-      if (hi) atomicAdd(&s->mass_hi[bin], hi);
+  r.each([&](const float (&l)[4], int i) {
+    uint32_t k[4];
+    bool in[4], any = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      k[j] = key_of(l[j]);
+      in[j] = k[j] <= b.hi && (k[j] >= b.lo || rest) && r.kept(k[j], r.base + i + j);
+      any |= in[j];
+    }
+    if (!any) return;
+    double w[4];
+    if (MASS) r.weights(l, w);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (!in[j]) continue;
+      u64 m = 0;
+      if (MASS) m = r.units(w[j]);
+      if (MASS && rest) all += m;
+      if (k[j] < b.lo) continue;
+      const int bin = b(l[j], k[j]);
+      atomicAdd(&s->cnt[bin], 1u);
+      if (MASS) {
+        const uint32_t lo = (uint32_t)m, old = atomicAdd(&s->mass_lo[bin], lo);
+        const uint32_t hi = (uint32_t)(m >> 32) + (old + lo < old);
+        if (hi) atomicAdd(&s->mass_hi[bin], hi);
+      }
     }
   });
   if (MASS && rest) {
@@ -323,21 +377,18 @@ __device__ void level(R& r, const Bins& b, uint32_t above, u64 mass_above, doubl
   r.sync();
 }
 
-// Kept candidates whose bin is `bin` (or above it too) go to the first CTA's list.
-template <typename R>
-__device__ void gather(R& r, const Bins& b, int bin, bool above_too) {
+// Kept candidates that `take(logit, key)` names go to the first CTA's list.
+template <typename R, typename F>
+__device__ void gather(R& r, F take) {
   Shared* first = r.peer(0);
-  r.each([&](float l, int i) {
-    const uint32_t k = key_of(l);
-    if (k < b.lo || !r.kept(k, r.base + i)) return;
-    if (k > b.hi) {
-      if (!above_too) return;
-    } else {
-      const int at = b(l, k);
-      if (above_too ? at > bin : at != bin) return;
+  r.each([&](const float (&l)[4], int i) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t k = key_of(l[j]);
+      if (!take(l[j], k) || !r.kept(k, r.base + i + j)) continue;
+      const uint32_t slot = atomicAdd(&first->n_list, 1u);
+      if (slot < kCap) first->list[slot] = ((u64)~k << 32) | (uint32_t)(r.base + i + j);
     }
-    const uint32_t slot = atomicAdd(&first->n_list, 1u);
-    if (slot < kCap) first->list[slot] = ((u64)~k << 32) | (uint32_t)(r.base + i);
   });
   r.sync();
 }
@@ -350,9 +401,12 @@ __device__ void sort_list(R& r, int n) {
   while (size < n) size *= 2;
   for (int i = n + r.tid; i < size; i += kNT) s->list[i] = ~0ull;
   __syncthreads();
+  // thread t compares the pair at a = 2t with bit j cleared: with j <= 32 a
+  // warp's pairs are its own 64 entries, and only wider steps meet the others
+  const int t = r.tid;
   for (int k = 2; k <= size; k *= 2)
     for (int j = k / 2; j > 0; j /= 2) {
-      for (int t = r.tid; t < size / 2; t += kNT) {
+      if (t < size / 2) {
         const int a = 2 * t - (t & (j - 1)), b = a + j;
         const u64 x = s->list[a], y = s->list[b];
         if ((x > y) == ((a & k) == 0)) {
@@ -360,8 +414,9 @@ __device__ void sort_list(R& r, int n) {
           s->list[b] = x;
         }
       }
-      __syncthreads();
+      if (j > 32 || (j == 1 && k >= 64)) __syncthreads(); else __syncwarp();
     }
+  __syncthreads();
 }
 
 // Inclusive sums of weight[0, n) in place (one CTA, two neighbours a thread).
@@ -440,7 +495,10 @@ __device__ void limit_ties(R& r, uint32_t key, uint32_t want) {
   Shared* s = r.s;
   const int per = r.slice / kWarps, i0 = r.warp * per;
   uint32_t c = 0;
-  r.each(i0, i0 + per, r.lane, 32, [&](float l, int i) { c += key_of(l) == key && r.kept(key, r.base + i); });
+  r.each(i0, i0 + per, r.lane, 32, [&](const float (&l)[4], int i) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c += key_of(l[j]) == key && r.kept(key, r.base + i + j);
+  });
   c = r.warp_add(c);
   __syncthreads();
   if (r.lane == 0) s->warp_u32[0][r.warp] = c;
@@ -495,12 +553,12 @@ __device__ bool select(R& r, uint32_t lo, double goal, int k, double tp, double 
       return false;
     }
     if (f.above + f.in <= kCap) {
-      gather(r, b, f.bin, true);
+      gather(r, [&](float l, uint32_t q) { return q > b.hi || (q >= b.lo && b(l, q) <= f.bin); });
       if (r.rank == 0) finish_list(r, (int)(f.above + f.in), MASS ? INT32_MAX : k, tp, mp, u, total, token, logprob);
       return true;
     }
     if (f.in <= kCap) {
-      gather(r, b, f.bin, false);
+      gather(r, [&](float l, uint32_t q) { return q <= b.hi && q >= b.lo && b(l, q) == f.bin; });
       if (r.rank == 0) {
         const int n = (int)f.in;
         sort_list(r, n);
@@ -524,11 +582,14 @@ __device__ bool select(R& r, uint32_t lo, double goal, int k, double tp, double 
     }
     // too many: their smallest and largest key bound the next level
     uint32_t kl = 0xffffffffu, kh = 0;
-    r.each([&](float l, int i) {
-      const uint32_t q = key_of(l);
-      if (q < b.lo || q > b.hi || !r.kept(q, r.base + i) || b(l, q) != f.bin) return;
-      kl = min(kl, q);
-      kh = max(kh, q);
+    r.each([&](const float (&l)[4], int i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t q = key_of(l[j]);
+        if (q < b.lo || q > b.hi || !r.kept(q, r.base + i + j) || b(l[j], q) != f.bin) continue;
+        kl = min(kl, q);
+        kh = max(kh, q);
+      }
     });
     kl = __reduce_min_sync(0xffffffffu, kl);
     kh = __reduce_max_sync(0xffffffffu, kh);
@@ -591,6 +652,8 @@ __global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
   r.row = static_cast<const T*>(p.logits) + b * p.row_stride + r.base;
   r.n = max(0, min(p.slice, p.V - r.base));
 
+  if (r.tid < 64) s->exp2_table[r.tid] = exp2((double)r.tid * (1.0 / 64));
+
   // ---- the slice's maximum (and the slice into shared memory), four vectors
   //      in flight a thread
   uint32_t mine = 0;
@@ -626,35 +689,33 @@ __global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
   const double tp = p.top_p ? p.top_p[b] : p.top_p0, mp = p.min_p ? p.min_p[b] : p.min_p0;
   if (!(temp > 0.f)) k = 1;
 
-  // maximum of the row; the least maximum over the warps and over the threads
-  // (of that many disjoint sets) bounds as many largest logits from below
-  const uint32_t wmax = __reduce_max_sync(0xffffffffu, mine), wmin = __reduce_min_sync(0xffffffffu, mine);
-  if (r.lane == 0) {
-    s->warp_u32[0][r.warp] = wmax;
-    s->warp_u32[1][r.warp] = wmin;
+  // Maximum of the row. And, for sets of 32, 16, .. 1 threads: the least
+  // maximum over the sets. As many logits as there are sets are at least that
+  // large, which bounds the k-th largest from below.
+  uint32_t set = mine;
+#pragma unroll
+  for (int g = kGroups - 1; g >= 0; --g) {  // sets of 32 >> g threads
+    const uint32_t least = __reduce_min_sync(0xffffffffu, set);
+    if (r.lane == 0) s->warp_u32[1 + g][r.warp] = least;
+    if (g) set = max(set, __shfl_xor_sync(0xffffffffu, set, 32 >> g));
   }
-  if (r.tid == 0) s->first = INT32_MAX;
+  if (r.lane == 0) s->warp_u32[0][r.warp] = set;
+  if (r.tid == 0) {
+    s->first = INT32_MAX;
+    s->n_list = 0;
+  }
   __syncthreads();
-  if (r.warp == 0) {
-    const bool have = r.lane < kWarps;
-    const uint32_t mx = __reduce_max_sync(0xffffffffu, have ? s->warp_u32[0][r.lane] : 0u);
-    const uint32_t mw = __reduce_min_sync(0xffffffffu, have ? s->warp_u32[0][r.lane] : 0xffffffffu);
-    const uint32_t mt = __reduce_min_sync(0xffffffffu, have ? s->warp_u32[1][r.lane] : 0xffffffffu);
+  if (r.warp <= kGroups) {
+    const uint32_t v = r.lane < kWarps ? s->warp_u32[r.warp][r.lane] : r.warp ? 0xffffffffu : 0u;
+    const uint32_t x = r.warp ? __reduce_min_sync(0xffffffffu, v) : __reduce_max_sync(0xffffffffu, v);
     if (r.lane < r.ctas) {
       Shared* o = r.peer(r.lane);
-      o->peer_max[r.rank] = mx;
-      o->peer_warp[r.rank] = mw;
-      o->peer_thread[r.rank] = mt;
+      (r.warp ? o->peer_least[r.warp - 1] : o->peer_max)[r.rank] = x;
     }
   }
   r.sync();
-  uint32_t least_w = 0xffffffffu, least_t = 0xffffffffu;
   r.mkey = 0;
-  for (int i = 0; i < r.ctas; ++i) {
-    r.mkey = max(r.mkey, s->peer_max[i]);
-    least_w = min(least_w, s->peer_warp[i]);
-    least_t = min(least_t, s->peer_thread[i]);
-  }
+  for (int i = 0; i < r.ctas; ++i) r.mkey = max(r.mkey, s->peer_max[i]);
   if (r.mkey == 0) {
     if (r.rank == 0 && r.tid == 0) {
       p.token[b] = -1;
@@ -668,8 +729,11 @@ __global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
 
   if (k == 1) {  // the lowest id of the largest logit
     int at = INT32_MAX;
-    r.each([&](float l, int i) {
-      if (key_of(l) == r.mkey) at = min(at, i + r.base);
+    const float top = (float)r.m;
+    r.each([&](const float (&l)[4], int i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (l[j] == top) at = min(at, i + j + r.base);
     });
     at = __reduce_min_sync(0xffffffffu, at);
     if (r.lane == 0 && at != INT32_MAX) atomicMin(&r.peer(0)->first, at);
@@ -681,7 +745,24 @@ __global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
     return;
   }
   if (k > 0 && k < p.V) {
-    uint32_t lo = k <= r.ctas * kWarps ? least_w : k <= r.ctas * kNT ? least_t : 0u;
+    int g = 0;  // the largest sets that are at least k
+    while (g < kGroups && (r.ctas * kWarps << g) < k) ++g;
+    uint32_t lo = 0;
+    if (g < kGroups) {
+      lo = 0xffffffffu;
+      for (int i = 0; i < r.ctas; ++i) lo = min(lo, s->peer_least[g][i]);
+    }
+    // About g ln g of the logits reach the least of g maxima, whatever their
+    // distribution: few enough for the list without a histogram.
+    if (lo && (r.ctas * kWarps << g) <= 128) {
+      gather(r, [&](float, uint32_t q) { return q >= lo; });
+      const uint32_t found = r.peer(0)->n_list;
+      if (r.ctas > 1) r.sync();  // read before the first CTA goes on
+      if (found <= kCap) {
+        if (r.rank == 0) finish_list(r, (int)found, k, tp, mp, u, 0, p.token + b, p.logprob + b);
+        return;
+      }
+    }
     if (lo == 0) lo = 1;  // an empty set among them: no bound
     if (select<false>(r, lo, (double)k, k, tp, mp, u, p.token + b, p.logprob + b)) return;
   }
@@ -699,16 +780,22 @@ __global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
   const int per = p.slice / kWarps, i0 = r.warp * per;
   // logits this low have w < mp for certain
   const float low = mp > 0.0 ? (float)(r.m + log2(mp) / r.c * 1.0001 - fabs(r.m) * 3e-7) : -INFINITY;
-  auto share = [&](float l, int i, double* w) -> u64 {
+  auto may = [&](float l, int i) {
     const uint32_t q = key_of(l);
-    if ((q != r.mkey && l < low) || !r.kept(q, r.base + i)) return 0;
-    *w = r.weight(l);
-    return *w >= mp || q == r.mkey ? r.units(*w) : 0;
+    return (l >= low || q == r.mkey) && r.kept(q, r.base + i);
   };
+  auto share = [&](float l, double w) { return w >= mp || l == (float)r.m ? r.units(w) : 0; };
   u64 sum = 0;
-  r.each(i0, i0 + per, r.lane, 32, [&](float l, int i) {
-    double w;
-    sum += share(l, i, &w);
+  r.each(i0, i0 + per, r.lane, 32, [&](const float (&l)[4], int i) {
+    bool in[4], any = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) any |= in[j] = may(l[j], i + j);
+    if (!any) return;
+    double w[4];
+    r.weights(l, w);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (in[j]) sum += share(l[j], w[j]);
   });
   sum = r.warp_add(sum);
   __syncthreads();
@@ -743,8 +830,8 @@ __global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
   before = s->peer_total[0];
   sum = 0;
   for (int i = p0 + r.lane; i < p1; i += 32) {
-    double w;
-    sum += share(r.at(i), i, &w);
+    const float l = r.at(i);
+    if (may(l, i)) sum += share(l, r.weight(l));
   }
   sum = r.warp_add(sum);
   __syncthreads();
@@ -753,8 +840,9 @@ __global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
   for (int i = 0; i < r.warp; ++i) before += s->warp_sum[i];
   if (!holds(before, sum)) return;
   for (int i = p0; i < p1; i += 32) {
-    double w = 0.0;
-    const u64 own = share(r.at(i + r.lane), i + r.lane, &w);  // blocks are whole warps wide
+    const float l = r.at(i + r.lane);  // blocks are whole warps wide
+    const double w = r.weight(l);
+    const u64 own = may(l, i + r.lane) ? share(l, w) : 0;
     u64 x = own;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
