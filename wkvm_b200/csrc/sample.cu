@@ -29,6 +29,7 @@
 // the whole row. HBM is read once: later passes find short slices in shared
 // memory and long ones in L2 (148 rows of 65,536 fp32 logits are 39 MB).
 #include <cooperative_groups.h>
+#include <float.h>
 
 #include <atomic>
 
@@ -64,23 +65,14 @@ constexpr int kGroups = 6;        // sets of 32, 16, .. 1 threads
 constexpr int kMaxCtas = 8;       // CTAs of a row (portable cluster size)
 constexpr int kSmemSlice = 16384; // logits of a slice kept in shared memory (two CTAs an SM)
 
-// Ascending unsigned order of floats; -inf is 0 and never kept (NaN and -0
-// are gone by then).
+// Ascending unsigned order of floats; -0 counts as 0, -inf and NaN as 0u.
 __device__ __forceinline__ uint32_t key_of(float x) {
-  if (x == -INFINITY) return 0u;
-  const uint32_t b = __float_as_uint(x);
+  if (!(x > -INFINITY)) return 0u;
+  const uint32_t b = __float_as_uint(x + 0.f);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 __device__ __forceinline__ float value_of(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
-}
-
-// fp32 to fp64 by the bits: the conversion instruction has a quarter of the
-// fp64 pipe's rate. Zero and subnormals become 2^-127 or so, infinities 2^128;
-// both are as good here.
-__device__ __forceinline__ double widen(float x) {
-  const uint32_t b = __float_as_uint(x);
-  return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));
 }
 
 // 2^t for -1000 < t <= 0, to 1e-13: with k = t rounded to 1/64 and r the rest,
@@ -125,7 +117,7 @@ struct alignas(16) Shared {
   u64 peer_mass[kMaxCtas], peer_total[kMaxCtas];
   Found found;
   uint32_t n_list;
-  uint32_t tau;                     // the last kept key
+  float tau;                        // the last kept logit
   int32_t limit;                    // ids below it are kept among its equals
   int32_t first;                    // greedy
   int32_t owner;                    // the warp whose block holds the drawn token
@@ -137,36 +129,30 @@ template <typename T, bool SMEM>
 struct Row {
   static constexpr int kVec = 16 / sizeof(T);
   Shared* s;
-  const float* vals;  // SMEM: the slice, NaN and -0 replaced
+  const float* vals;  // SMEM: the slice
   const T* row;       // the slice in global memory
   bool vec;           // it starts on 16 bytes
   int rank, ctas, tid, lane, warp, slice, base;  // base: the slice's first id
   int n;              // logits of the slice that exist
-  double m, c;       // maximum; log2(e) / temperature
+  float top;         // the row's maximum
+  bool flat;         // it is +inf: only logits equal to it are kept, all of weight 1
+  double c;          // log2(e) / temperature
   double shift;      // of units(), a power of two >= 1
-  uint32_t mkey;
-  uint32_t tau;      // kept: key > tau, or key == tau and id < limit
+  // kept: l > tau, or l == tau and id < limit (NaN and -inf never are)
+  float tau;
   int32_t limit;
 
-  // Four at once: a weight is a chain of some twenty dependent fp64
-  // operations, and only other chains fill its latency.
+  // Weights of four kept logits (others give any value). Four at once: each is
+  // a chain of dependent fp64 operations, and only other chains fill its latency.
   template <int W>
   __device__ __forceinline__ void weights(const float (&l)[W], double (&w)[W]) const {
-    double t[W];
-    bool in[W];
 #pragma unroll
     for (int j = 0; j < W; ++j) {
-      t[j] = (widen(l[j]) - m) * c;
-      // below 2^-54 is less than half a unit: by the exponent and top mantissa
-      // bits, t > -54 (NaN and -inf, of a maximum of inf, are not)
-      in[j] = (uint32_t)__double2hiint(t[j]) < 0xc04b0000u;
-    }
-#pragma unroll
-    for (int j = 0; j < W; ++j) w[j] = exp2_neg(in[j] ? t[j] : -54.0, s->exp2_table);
-#pragma unroll
-    for (int j = 0; j < W; ++j) {
-      w[j] = in[j] ? w[j] : 0.0;
-      w[j] = l[j] == (float)m ? 1.0 : w[j];
+      const double t = ((double)l[j] - (double)top) * c;
+      // t <= 0, at least about -60: that is no unit any more. Negative numbers
+      // ascend with their bits, so the upper word's smaller one is taken.
+      const uint32_t hi = min((uint32_t)__double2hiint(t), 0xc04e0000u);
+      w[j] = flat ? 1.0 : exp2_neg(__hiloint2double((int)hi, __double2loint(t)), s->exp2_table);
     }
   }
   __device__ __forceinline__ double weight(float l) const {
@@ -176,17 +162,15 @@ struct Row {
     return w[0];
   }
   __device__ u64 units(double w) const {
-    return (u64)(__double_as_longlong(w + shift) - __double_as_longlong(shift));
+    const double x = w + shift;
+    return (u64)(uint32_t)(__double2hiint(x) - __double2hiint(shift)) << 32 | (uint32_t)__double2loint(x);
   }
   __device__ double weight_of(u64 z) const { return (double)z * (shift * 0x1p-52); }
-  __device__ u64 mass(float l) const { return units(weight(l)); }
-  __device__ bool kept(uint32_t k, int id) const { return k > tau || (k == tau && id < limit); }
+  __device__ __forceinline__ bool kept(float l, int id) const { return l > tau || (l == tau && id < limit); }
 
-  // NaN counts as -inf, -0 as 0
-  __device__ static float clean(float v) { return v > -INFINITY ? v + 0.f : -INFINITY; }
   __device__ float at(int i) const {
     if constexpr (SMEM) return vals[i];
-    return i < n ? clean(to_f32(row[i])) : -INFINITY;
+    return i < n ? to_f32(row[i]) : -INFINITY;
   }
   // f(logits, i) for the logits [i0, i1) four at a time, i the first one's
   // index, dealt to `nt` threads of which this is thread t. Past the slice's
@@ -211,7 +195,7 @@ struct Row {
         for (int h = 0; h < kVec; h += 4) {
           float l[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) l[j] = clean(to_f32(reinterpret_cast<const T*>(&q)[h + j]));
+          for (int j = 0; j < 4; ++j) l[j] = to_f32(reinterpret_cast<const T*>(&q)[h + j]);
           f(l, i + h);
         }
       }
@@ -248,26 +232,26 @@ struct Row {
   }
 };
 
-// A level's bins: keys [lo, hi] into kBins bins, the largest first. Linear in
-// the logit where that is safe, else linear in the key; any monotone map does.
+// A level's bins: logits [lo, hi] into kBins bins, the largest first. Linear
+// in the logit where that is safe, else in the key; any monotone map does.
 struct Bins {
-  uint32_t lo, hi;
-  float top, scale;  // scale 0: linear in the key
-  u64 step;          // ceil(2^32 bins / keys)
-  __device__ Bins(uint32_t l, uint32_t h) : lo(l), hi(h), top(value_of(h)), scale(0.f), step(0) {
-    const float range = top - value_of(l);
+  float lo, hi, scale;  // scale 0: linear in the key
+  u64 step;             // 2^32 bins / keys
+  __device__ Bins(float l, float h) : lo(l), hi(h), scale(0.f), step(0) {
+    const float range = hi - lo;
     if (range > 1e-30f && range < 1e30f)
       scale = kBins / range;
     else
-      step = ((u64)kBins << 32) / ((u64)(h - l) + 1);
+      step = ((u64)kBins << 32) / ((u64)(key_of(hi) - key_of(lo)) + 1);
   }
-  __device__ int operator()(float l, uint32_t k) const {
-    const int b = scale > 0.f ? (int)((top - l) * scale) : (int)(((u64)(hi - k) * step) >> 32);
+  __device__ __forceinline__ bool holds(float l) const { return l >= lo && l <= hi; }
+  __device__ __forceinline__ int operator()(float l) const {
+    const int b = scale > 0.f ? (int)((hi - l) * scale) : (int)(((u64)(key_of(hi) - key_of(l)) * step) >> 32);
     return b < kBins - 1 ? b : kBins - 1;
   }
 };
 
-// One level: histogram of the kept candidates with keys in [b.lo, b.hi], and
+// One level: histogram of the kept candidates in [b.lo, b.hi], and
 // the first bin at which above + the running count (or mass) reaches the goal.
 // `rest`: mass of what is kept below b.lo joins the total, and the goal is
 // share times that total (first level of top-p). Two cluster barriers.
@@ -282,14 +266,9 @@ __device__ void level(R& r, const Bins& b, uint32_t above, u64 mass_above, doubl
   __syncthreads();
   u64 all = 0;
   r.each([&](const float (&l)[4], int i) {
-    uint32_t k[4];
     bool in[4], any = false;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      k[j] = key_of(l[j]);
-      in[j] = k[j] <= b.hi && (k[j] >= b.lo || rest) && r.kept(k[j], r.base + i + j);
-      any |= in[j];
-    }
+    for (int j = 0; j < 4; ++j) any |= in[j] = l[j] <= b.hi && (rest || l[j] >= b.lo) && r.kept(l[j], r.base + i + j);
     if (!any) return;
     double w[4];
     if (MASS) r.weights(l, w);
@@ -299,8 +278,8 @@ __device__ void level(R& r, const Bins& b, uint32_t above, u64 mass_above, doubl
       u64 m = 0;
       if (MASS) m = r.units(w[j]);
       if (MASS && rest) all += m;
-      if (k[j] < b.lo) continue;
-      const int bin = b(l[j], k[j]);
+      if (l[j] < b.lo) continue;
+      const int bin = b(l[j]);
       atomicAdd(&s->cnt[bin], 1u);
       if (MASS) {
         const uint32_t lo = (uint32_t)m, old = atomicAdd(&s->mass_lo[bin], lo);
@@ -324,12 +303,18 @@ __device__ void level(R& r, const Bins& b, uint32_t above, u64 mass_above, doubl
     // two neighbouring bins a thread, summed over the cluster
     uint32_t c[2] = {0, 0};
     u64 m[2] = {0, 0};
-    for (int p = 0; p < r.ctas; ++p) {
-      const Shared* o = r.peer(p);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        c[j] += o->cnt[2 * r.tid + j];
-        if (MASS) m[j] += o->mass_lo[2 * r.tid + j] + ((u64)o->mass_hi[2 * r.tid + j] << 32);
+    for (int p = 0; p < kMaxCtas; ++p) {  // every peer's bins in flight at once
+      if (p >= r.ctas) break;
+      const Shared* o = r.peer(p);
+      const uint2 n = *reinterpret_cast<const uint2*>(&o->cnt[2 * r.tid]);
+      c[0] += n.x;
+      c[1] += n.y;
+      if (MASS) {
+        const uint2 lo = *reinterpret_cast<const uint2*>(&o->mass_lo[2 * r.tid]);
+        const uint2 hi = *reinterpret_cast<const uint2*>(&o->mass_hi[2 * r.tid]);
+        m[0] += (u64)hi.x << 32 | lo.x;
+        m[1] += (u64)hi.y << 32 | lo.y;
       }
     }
     uint32_t cs = c[0] + c[1];
@@ -377,17 +362,16 @@ __device__ void level(R& r, const Bins& b, uint32_t above, u64 mass_above, doubl
   r.sync();
 }
 
-// Kept candidates that `take(logit, key)` names go to the first CTA's list.
+// Kept candidates that `take(logit)` names go to the first CTA's list.
 template <typename R, typename F>
 __device__ void gather(R& r, F take) {
   Shared* first = r.peer(0);
   r.each([&](const float (&l)[4], int i) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint32_t k = key_of(l[j]);
-      if (!take(l[j], k) || !r.kept(k, r.base + i + j)) continue;
+      if (!take(l[j]) || !r.kept(l[j], r.base + i + j)) continue;
       const uint32_t slot = atomicAdd(&first->n_list, 1u);
-      if (slot < kCap) first->list[slot] = ((u64)~k << 32) | (uint32_t)(r.base + i + j);
+      if (slot < kCap) first->list[slot] = ((u64)~key_of(l[j]) << 32) | (uint32_t)(r.base + i + j);
     }
   });
   r.sync();
@@ -463,7 +447,7 @@ __device__ void finish_list(R& r, int n, int k, double tp, double mp, double u, 
   }
   if (mp > 0.0) {
     uint32_t stay = 0;
-    for (int i = r.tid; i < n; i += kNT) stay += i == 0 || weigh(i) >= mp || list_key(s->list[i]) == r.mkey;
+    for (int i = r.tid; i < n; i += kNT) stay += i == 0 || weigh(i) >= mp || value_of(list_key(s->list[i])) == r.top;
     n = (int)r.block_add(stay);
   }
   // draw in order of ids
@@ -489,15 +473,15 @@ __device__ void finish_list(R& r, int n, int k, double tp, double mp, double u, 
   }
 }
 
-// Keeps, of the kept candidates that equal `key`, the `want` lowest ids.
+// Keeps, of the kept candidates that equal `tie`, the `want` lowest ids.
 template <typename R>
-__device__ void limit_ties(R& r, uint32_t key, uint32_t want) {
+__device__ void limit_ties(R& r, float tie, uint32_t want) {
   Shared* s = r.s;
   const int per = r.slice / kWarps, i0 = r.warp * per;
   uint32_t c = 0;
   r.each(i0, i0 + per, r.lane, 32, [&](const float (&l)[4], int i) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) c += key_of(l[j]) == key && r.kept(key, r.base + i + j);
+    for (int j = 0; j < 4; ++j) c += l[j] == tie && r.kept(tie, r.base + i + j);
   });
   c = r.warp_add(c);
   __syncthreads();
@@ -514,7 +498,7 @@ __device__ void limit_ties(R& r, uint32_t key, uint32_t want) {
   for (int w = 0; w < r.warp; ++w) before += s->warp_u32[0][w];
   if (before < want && before + s->warp_u32[0][r.warp] >= want) {  // one warp of the cluster
     for (int i = i0; i < i0 + per; i += 32) {
-      const bool is = key_of(r.at(i + r.lane)) == key && r.kept(key, r.base + i + r.lane);
+      const bool is = r.at(i + r.lane) == tie && r.kept(tie, r.base + i + r.lane);
       const uint32_t b = __ballot_sync(0xffffffffu, is);
       if (before + __popc(b) < want) {
         before += __popc(b);
@@ -527,7 +511,7 @@ __device__ void limit_ties(R& r, uint32_t key, uint32_t want) {
     }
   }
   r.sync();
-  r.tau = key;
+  r.tau = tie;
   r.limit = s->limit;
 }
 
@@ -535,10 +519,10 @@ __device__ void limit_ties(R& r, uint32_t key, uint32_t want) {
 // count reaches `goal` (or whose mass reaches tp of the mass of all kept).
 // Returns true when the row was finished on the list.
 template <bool MASS, typename R>
-__device__ bool select(R& r, uint32_t lo, double goal, int k, double tp, double mp, double u,
+__device__ bool select(R& r, float lo, double goal, int k, double tp, double mp, double u,
                        int64_t* token, float* logprob) {
   Shared* s = r.s;
-  Bins b(lo, r.mkey);
+  Bins b(lo, r.top);
   uint32_t above = 0;
   u64 mass_above = 0, total = 0;
   for (bool first = true;; first = false) {
@@ -549,20 +533,20 @@ __device__ bool select(R& r, uint32_t lo, double goal, int k, double tp, double 
     // of (a share of nothing), the top alone is kept
     if (f.bin < 0) {
       if (!MASS) return false;
-      limit_ties(r, r.mkey, 1);
+      limit_ties(r, r.top, 1);
       return false;
     }
     if (f.above + f.in <= kCap) {
-      gather(r, [&](float l, uint32_t q) { return q > b.hi || (q >= b.lo && b(l, q) <= f.bin); });
+      gather(r, [&](float l) { return l > b.hi || (l >= b.lo && b(l) <= f.bin); });
       if (r.rank == 0) finish_list(r, (int)(f.above + f.in), MASS ? INT32_MAX : k, tp, mp, u, total, token, logprob);
       return true;
     }
     if (f.in <= kCap) {
-      gather(r, [&](float l, uint32_t q) { return q <= b.hi && q >= b.lo && b(l, q) == f.bin; });
+      gather(r, [&](float l) { return b.holds(l) && b(l) == f.bin; });
       if (r.rank == 0) {
         const int n = (int)f.in;
         sort_list(r, n);
-        for (int i = r.tid; i < n; i += kNT) s->weight[i] = MASS ? r.mass(value_of(list_key(s->list[i]))) : 1;
+        for (int i = r.tid; i < n; i += kNT) s->weight[i] = MASS ? r.units(r.weight(value_of(list_key(s->list[i])))) : 1;
         __syncthreads();
         scan_weights(r, n);
         const u64 base = MASS ? f.mass_above : f.above;
@@ -570,7 +554,7 @@ __device__ bool select(R& r, uint32_t lo, double goal, int k, double tp, double 
           const double before = (double)(base + (i ? s->weight[i - 1] : 0));
           if (before < goal && ((double)(base + s->weight[i]) >= goal || i == n - 1))
             for (int p = 0; p < r.ctas; ++p) {
-              r.peer(p)->tau = list_key(s->list[i]);
+              r.peer(p)->tau = value_of(list_key(s->list[i]));
               r.peer(p)->limit = (int32_t)(uint32_t)s->list[i] + 1;
             }
         }
@@ -585,10 +569,9 @@ __device__ bool select(R& r, uint32_t lo, double goal, int k, double tp, double 
     r.each([&](const float (&l)[4], int i) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t q = key_of(l[j]);
-        if (q < b.lo || q > b.hi || !r.kept(q, r.base + i + j) || b(l[j], q) != f.bin) continue;
-        kl = min(kl, q);
-        kh = max(kh, q);
+        if (!b.holds(l[j]) || !r.kept(l[j], r.base + i + j) || b(l[j]) != f.bin) continue;
+        kl = min(kl, key_of(l[j]));
+        kh = max(kh, key_of(l[j]));
       }
     });
     kl = __reduce_min_sync(0xffffffffu, kl);
@@ -615,17 +598,17 @@ __device__ bool select(R& r, uint32_t lo, double goal, int k, double tp, double 
     if (kl == kh) {  // equal logits: as many as it takes
       uint32_t want = (uint32_t)(goal - (double)f.above);
       if (MASS) {
-        const u64 w = r.mass(value_of(kl));
+        const u64 w = r.units(r.weight(value_of(kl)));
         want = (uint32_t)fmin((goal - (double)f.mass_above) / (double)w, (double)(f.in - 1)) ;
         while (want > 0 && (double)(f.mass_above + (want - 1) * w) >= goal) --want;
         while (want < f.in && (double)(f.mass_above + want * w) < goal) ++want;
       }
-      limit_ties(r, kl, want);
+      limit_ties(r, value_of(kl), want);
       return false;
     }
     above = f.above;
     mass_above = f.mass_above;
-    b = Bins(kl, kh);
+    b = Bins(value_of(kl), value_of(kh));
   }
 }
 
@@ -645,7 +628,7 @@ __global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
   r.warp = r.tid >> 5;
   r.slice = p.slice;
   r.base = r.rank * p.slice;
-  r.tau = 0;  // key 0 is never kept
+  r.tau = -INFINITY;
   r.limit = 0;
   r.vec = p.vec;
   const int b = blockIdx.x / p.ctas;
@@ -656,11 +639,10 @@ __global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
 
   // ---- the slice's maximum (and the slice into shared memory), four vectors
   //      in flight a thread
-  uint32_t mine = 0;
+  float most = -INFINITY;
   auto put = [&](int i, float v) {
-    v = R::clean(v);
     if constexpr (SMEM) vals[i] = v;
-    mine = max(mine, key_of(v));
+    most = fmaxf(most, v);  // not NaN
   };
   constexpr int kFly = 4;
   const int whole = p.vec ? r.n / kVec * kVec : 0;
@@ -692,7 +674,7 @@ __global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
   // Maximum of the row. And, for sets of 32, 16, .. 1 threads: the least
   // maximum over the sets. As many logits as there are sets are at least that
   // large, which bounds the k-th largest from below.
-  uint32_t set = mine;
+  uint32_t set = key_of(most);
 #pragma unroll
   for (int g = kGroups - 1; g >= 0; --g) {  // sets of 32 >> g threads
     const uint32_t least = __reduce_min_sync(0xffffffffu, set);
@@ -714,26 +696,30 @@ __global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
     }
   }
   r.sync();
-  r.mkey = 0;
-  for (int i = 0; i < r.ctas; ++i) r.mkey = max(r.mkey, s->peer_max[i]);
-  if (r.mkey == 0) {
+  uint32_t top = 0;
+  for (int i = 0; i < r.ctas; ++i) top = max(top, s->peer_max[i]);
+  if (top == 0) {
     if (r.rank == 0 && r.tid == 0) {
       p.token[b] = -1;
       p.logprob[b] = -INFINITY;
     }
     return;
   }
-  r.m = value_of(r.mkey);
+  r.top = value_of(top);
+  r.flat = r.top == INFINITY;
+  if (r.flat) {
+    r.tau = r.top;
+    r.limit = INT32_MAX;
+  }
   r.c = 1.4426950408889634 / (double)temp;
   r.shift = p.shift;
 
   if (k == 1) {  // the lowest id of the largest logit
     int at = INT32_MAX;
-    const float top = (float)r.m;
     r.each([&](const float (&l)[4], int i) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (l[j] == top) at = min(at, i + j + r.base);
+        if (l[j] == r.top) at = min(at, i + j + r.base);
     });
     at = __reduce_min_sync(0xffffffffu, at);
     if (r.lane == 0 && at != INT32_MAX) atomicMin(&r.peer(0)->first, at);
@@ -747,44 +733,41 @@ __global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
   if (k > 0 && k < p.V) {
     int g = 0;  // the largest sets that are at least k
     while (g < kGroups && (r.ctas * kWarps << g) < k) ++g;
-    uint32_t lo = 0;
+    uint32_t least = 0;
     if (g < kGroups) {
-      lo = 0xffffffffu;
-      for (int i = 0; i < r.ctas; ++i) lo = min(lo, s->peer_least[g][i]);
+      least = 0xffffffffu;
+      for (int i = 0; i < r.ctas; ++i) least = min(least, s->peer_least[g][i]);
     }
+    const float lo = least ? value_of(least) : -FLT_MAX;  // 0: an empty set among them
     // About g ln g of the logits reach the least of g maxima, whatever their
     // distribution: few enough for the list without a histogram.
-    if (lo && (r.ctas * kWarps << g) <= 128) {
-      gather(r, [&](float, uint32_t q) { return q >= lo; });
+    if (least && (r.ctas * kWarps << g) <= 128) {
+      gather(r, [&](float l) { return l >= lo; });
       const uint32_t found = r.peer(0)->n_list;
-      if (r.ctas > 1) r.sync();  // read before the first CTA goes on
+      r.sync();  // read before the first CTA goes on
       if (found <= kCap) {
         if (r.rank == 0) finish_list(r, (int)found, k, tp, mp, u, 0, p.token + b, p.logprob + b);
         return;
       }
     }
-    if (lo == 0) lo = 1;  // an empty set among them: no bound
     if (select<false>(r, lo, (double)k, k, tp, mp, u, p.token + b, p.logprob + b)) return;
   }
   if (tp < 1.0) {
     // tokens of weight below (1 - p) / 2V hold less than 1 - p of the mass, as
     // the largest alone weighs 1: the boundary lies above them
     const double eps = (1.0 - tp) / (2.0 * (double)p.V);
-    const float bound = (float)(r.m + log2(eps) / r.c * 1.0001 - fabs(r.m) * 3e-7);
-    uint32_t lo = bound > -INFINITY ? key_of(bound) : 1u;
-    lo = max(min(lo, r.mkey), 1u);
+    const float bound = r.flat ? r.top : (float)(r.top + log2(eps) / r.c * 1.0001 - fabs((double)r.top) * 3e-7);
+    const float lo = bound > -FLT_MAX ? fminf(bound, r.top) : -FLT_MAX;
     if (select<true>(r, lo, 0.0, k, tp, mp, u, p.token + b, p.logprob + b)) return;
   }
 
   // ---- draw from the whole row: masses of contiguous blocks, one per warp
   const int per = p.slice / kWarps, i0 = r.warp * per;
   // logits this low have w < mp for certain
-  const float low = mp > 0.0 ? (float)(r.m + log2(mp) / r.c * 1.0001 - fabs(r.m) * 3e-7) : -INFINITY;
-  auto may = [&](float l, int i) {
-    const uint32_t q = key_of(l);
-    return (l >= low || q == r.mkey) && r.kept(q, r.base + i);
-  };
-  auto share = [&](float l, double w) { return w >= mp || l == (float)r.m ? r.units(w) : 0; };
+  const float low = mp > 0.0 && !r.flat
+                        ? (float)(r.top + log2(mp) / r.c * 1.0001 - fabs((double)r.top) * 3e-7) : -INFINITY;
+  auto may = [&](float l, int i) { return (l >= low || l == r.top) && r.kept(l, r.base + i); };
+  auto share = [&](float l, double w) { return w >= mp || l == r.top ? r.units(w) : 0; };
   u64 sum = 0;
   r.each(i0, i0 + per, r.lane, 32, [&](const float (&l)[4], int i) {
     bool in[4], any = false;
