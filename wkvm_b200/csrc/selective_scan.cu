@@ -12,6 +12,7 @@
 #include <float.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "ssm_common.cuh"
 
@@ -156,6 +157,16 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
   return r;
 }
 
+// softplus() of two
+__device__ __forceinline__ f32x2 softplus2(f32x2 x) {
+  const float2 v = unpack2(x);
+  const f32x2 e = pack2(ex2(-kLog2e * fabsf(v.x)), ex2(-kLog2e * fabsf(v.y)));
+  f32x2 q = pack2(log1p_coeff(8), log1p_coeff(8));
+#pragma unroll
+  for (int i = 7; i >= 0; --i) q = fma2(q, e, pack2(log1p_coeff(i), log1p_coeff(i)));
+  return fma2(q, e, pack2(fmaxf(v.x, 0.0f), fmaxf(v.y, 0.0f)));
+}
+
 template <typename T, int V>
 struct Raw {
   static constexpr int kBytes = sizeof(T) * V, kWords = (kBytes + 3) / 4;
@@ -163,18 +174,30 @@ struct Raw {
   __device__ __forceinline__ float f32(int i) const {
     if constexpr (sizeof(T) == 4) {
       return __uint_as_float(w[i]);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      // byte permutes: the compiler's shifts by multiplication would crowd the
+      // fp32 pipe
+      uint32_t x;
+      if (i % 2)
+        asm("prmt.b32 %0, %1, 0, 0x3244;" : "=r"(x) : "r"(w[i / 2]));
+      else
+        asm("prmt.b32 %0, %1, 0, 0x1044;" : "=r"(x) : "r"(w[i / 2]));
+      return __uint_as_float(x);
     } else {
       const uint16_t h = (uint16_t)(w[i / 2] >> (16 * (i % 2)));
       return to_f32(*reinterpret_cast<const T*>(&h));
     }
   }
-  __device__ __forceinline__ void set(int i, float x) {
-    const T t = from_f32<T>(x);
+  __device__ __forceinline__ void set2(int i, float x, float y) {  // elements i and i + 1, i even
     if constexpr (sizeof(T) == 4) {
-      w[i] = *reinterpret_cast<const uint32_t*>(&t);
+      w[i] = __float_as_uint(x);
+      w[i + 1] = __float_as_uint(y);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const __half2 h = __floats2half2_rn(x, y);
+      w[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
     } else {
-      const uint32_t h = *reinterpret_cast<const uint16_t*>(&t);
-      w[i / 2] = i % 2 ? (w[i / 2] & 0xffffu) | h << 16 : h;
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+      w[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
     }
   }
 };
@@ -211,23 +234,21 @@ __device__ __forceinline__ Raw<T, V> load_some(const T* p, int n) {
   return r;
 }
 
-// V elements from global to shared memory, zeros where there are none (n <= 0).
-// vec: src is aligned to the whole vector and n is at most 0 or at least V;
-// the copy is then asynchronous, for copies_done() to wait for.
+// V elements from global to shared memory, zeros unless `have`: asynchronous,
+// for copies_done() to wait for, where both sides are aligned to the vector.
 template <typename T, int V>
-__device__ __forceinline__ void copy_in(T* dst, const T* src, const T* safe, int n, bool vec) {
-  if (vec) {
-    const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
-    const T* from = n > 0 ? src : safe;
-    const int size = n > 0 ? Raw<T, V>::kBytes : 0;
-    if constexpr (Raw<T, V>::kBytes == 16)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(from), "r"(size) : "memory");
-    else
-      asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(from), "n"(Raw<T, V>::kBytes), "r"(size) : "memory");
-  } else {
-    const Raw<T, V> r = load_some<T, V>(src, n);
-    move<T, V>(reinterpret_cast<Raw<T, V>*>(dst), &r);
-  }
+__device__ __forceinline__ void copy_async(uint32_t dst, const T* src, bool have) {
+  const int size = have ? Raw<T, V>::kBytes : 0;
+  if constexpr (Raw<T, V>::kBytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(size) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(Raw<T, V>::kBytes), "r"(size) : "memory");
+}
+// The first n of V elements one by one, zeros for the others.
+template <typename T, int V>
+__device__ __forceinline__ void copy_some(T* dst, const T* src, int n) {
+  const Raw<T, V> r = load_some<T, V>(src, n);
+  move<T, V>(reinterpret_cast<Raw<T, V>*>(dst), &r);
 }
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
@@ -257,7 +278,7 @@ struct Tile {
   static constexpr int oP = oX + 2 * kStage;        // dt_bias and D of the channels
   static constexpr int oH = oP + 8 * CB;            // cluster: final states, step sums
   static constexpr int bytes(bool cluster) { return oH + (cluster ? 8 * NP * (NS + 1) * NT : 0); }
-  static_assert(EPT >= 2 && BPT >= 2 && TT * NT % CB == 0 && XB % 16 == 0 && BB % 16 == 0, "tile too small for the block");
+  static_assert(EPT >= 2 && BPT >= 2 && NT * VB % N == 0 && TT * NT % CB == 0 && XB % 16 == 0 && BB % 16 == 0, "tile too small for the block");
 };
 
 struct TileArgs {
@@ -349,167 +370,230 @@ __global__ void __launch_bounds__(NT) scan_tiles_kernel(TileArgs q) {
 
   // A thread copies in the elements it owns and is their only reader, so it
   // waits for its own copies alone; B and C, read by all, are also behind the
-  // barrier ahead of the main loop.
-  auto fetch = [&](int64_t t0, int stage, bool emit) {
-    T* s = reinterpret_cast<T*>(smem + K::oX + stage * K::kStage);
+  // barrier ahead of the main loop. Pointers run along with the tiles, which
+  // are fetched in order; past the end they stay on the tile's first token.
+  const int len = (int)sp.len;
+  constexpr int BT = NT * VB / N;  // tokens of one round of copies of B and C
+  const int tb = tid * VB / N;
+  const T *fx, *fd, *fz, *fb, *fc;
+  T* out;
+  int left;  // tokens from the next tile's start to the sequence's end
+  auto aim = [&](int t0) {
+    fx = xp + (int64_t)t0 * p.x.ts;
+    fd = dp + (int64_t)t0 * p.dt.ts;
+    fz = zp ? zp + (int64_t)t0 * p.z.ts : nullptr;
+    fb = bp + (int64_t)t0 * p.B.ts + tid * VB % N;
+    fc = cp + (int64_t)t0 * p.C.ts + tid * VB % N;
+    out = op + (int64_t)(t0 + te) * p.D;
+    left = len - t0;
+  };
+  auto fetch = [&](int stage, bool emit) {
+    T* sx = reinterpret_cast<T*>(smem + K::oX + stage * K::kStage) + te * CB + ce;
+    T* sb = reinterpret_cast<T*>(smem + K::oX + stage * K::kStage) + 3 * TT * CB + tid * VB;
+    if (q.vec_x) {
+      const uint32_t d = (uint32_t)__cvta_generic_to_shared(sx);
 #pragma unroll
-    for (int r = 0; r < RV; ++r) {
-      const int64_t t = t0 + te + r * TS;
-      const int k = t < sp.len ? nv : 0, at = (te + r * TS) * CB + ce;
-      copy_in<T, VE>(s + at, xp + t * p.x.ts, xp, k, q.vec_x);
-      copy_in<T, VE>(s + TT * CB + at, dp + t * p.dt.ts, dp, k, q.vec_x);
-      if (emit && zp) copy_in<T, VE>(s + 2 * TT * CB + at, zp + t * p.z.ts, zp, k, q.vec_x);
-    }
-    s += 3 * TT * CB;
+      for (int r = 0; r < RV; ++r) {
+        const bool have = te + r * TS < left && nv > 0;
+        const int t = have ? te + r * TS : 0;
+        const uint32_t at = d + r * TS * CB * (int)sizeof(T);
+        copy_async<T, VE>(at, nv > 0 ? fx + t * p.x.ts : xp - ce, have);
+        copy_async<T, VE>(at + K::XB, nv > 0 ? fd + t * p.dt.ts : dp - ce, have);
+        if (emit && zp) copy_async<T, VE>(at + 2 * K::XB, nv > 0 ? fz + t * p.z.ts : zp - ce, have);
+      }
+    } else {
 #pragma unroll
-    for (int r = 0; r < RB; ++r) {
-      const int e = (r * NT + tid) * VB;
-      const int64_t t = t0 + e / N;
-      const int k = t < sp.len ? VB : 0;
-      copy_in<T, VB>(s + e, bp + t * p.B.ts + e % N, bp, k, q.vec_b);
-      if (emit) copy_in<T, VB>(s + TT * N + e, cp + t * p.C.ts + e % N, cp, k, q.vec_b);
+      for (int r = 0; r < RV; ++r) {
+        const int64_t t = te + r * TS;
+        const int k = t < left ? nv : 0;
+        copy_some<T, VE>(sx + r * TS * CB, fx + t * p.x.ts, k);
+        copy_some<T, VE>(sx + TT * CB + r * TS * CB, fd + t * p.dt.ts, k);
+        if (emit && zp) copy_some<T, VE>(sx + 2 * TT * CB + r * TS * CB, fz + t * p.z.ts, k);
+      }
     }
+    if (q.vec_b) {
+      const uint32_t d = (uint32_t)__cvta_generic_to_shared(sb);
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        const bool have = tb + r * BT < left;
+        const int t = have ? tb + r * BT : 0;
+        copy_async<T, VB>(d + r * NT * VB * (int)sizeof(T), fb + t * p.B.ts, have);
+        if (emit) copy_async<T, VB>(d + K::BB + r * NT * VB * (int)sizeof(T), fc + t * p.C.ts, have);
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        const int64_t t = tb + r * BT;
+        const int k = t < left ? VB : 0;
+        copy_some<T, VB>(sb + r * NT * VB, fb + t * p.B.ts, k);
+        if (emit) copy_some<T, VB>(sb + TT * N + r * NT * VB, fc + t * p.C.ts, k);
+      }
+    }
+    fx += TT * p.x.ts;
+    fd += TT * p.dt.ts;
+    if (zp) fz += TT * p.z.ts;
+    fb += TT * p.B.ts;
+    fc += TT * p.C.ts;
+    left -= TT;
   };
 
   f32x2 steps[NP];  // sums of delta over the part (first pass of a cluster)
 #pragma unroll
   for (int j = 0; j < NP; ++j) steps[j] = 0;
-  auto run = [&](int64_t t0, int64_t t1, bool emit) {
+  const float* sp0 = sP + ce;
+  const float* dp0 = sD + padded(4 * ch);
+  float* dst0 = sD + te * K::DROW + padded(2 * ce);
+  const float* src0 = sY + te * K::YROW + padded(ce * L);
+  float* y0 = sY + padded(2 * tid);
+  auto run = [&](int t0, int t1, bool emit) {
     if (t0 >= t1) return;
-    fetch(t0, 0, emit);
+    aim(t0);
+    fetch(0, emit);
     meet();  // sP; the tiles of an earlier run
     for (int stage = 0; t0 < t1; t0 += TT, stage ^= 1) {
       const T* sX = reinterpret_cast<const T*>(smem + K::oX + stage * K::kStage);
+      const T* own = sX + te * CB + ce;
       const T* sB = sX + 3 * TT * CB;
       const T* sC = sB + TT * N;
       copies_done();
+      {
+        // tokens behind the end give any numbers here; the main loop stops
+        // ahead of them
+        Raw<T, VE> rx[RV], rd[RV];
 #pragma unroll
-      for (int r = 0; r < RV; ++r) {
-        const int t = te + r * TS;
-        const bool live = t0 + t < sp.len;
-        float* dst = sD + t * K::DROW + padded(2 * ce);
-        Raw<T, VE> rx, rd;
-        move<T, VE>(&rx, reinterpret_cast<const Raw<T, VE>*>(sX + t * CB + ce));
-        move<T, VE>(&rd, reinterpret_cast<const Raw<T, VE>*>(sX + TT * CB + t * CB + ce));
+        for (int r = 0; r < RV; ++r) {
+          move<T, VE>(&rx[r], reinterpret_cast<const Raw<T, VE>*>(own + r * TS * CB));
+          move<T, VE>(&rd[r], reinterpret_cast<const Raw<T, VE>*>(own + TT * CB + r * TS * CB));
+        }
 #pragma unroll
         for (int i = 0; i < VE; i += 2) {
-          const float2 bias = *reinterpret_cast<const float2*>(sP + ce + i);
-          float d0 = rd.f32(i) + bias.x, d1 = rd.f32(i + 1) + bias.y;
-          if (p.softplus) {
-            d0 = softplus(d0);
-            d1 = softplus(d1);
+          const f32x2 bias = *reinterpret_cast<const f32x2*>(sp0 + i);
+#pragma unroll
+          for (int r = 0; r < RV; ++r) {
+            f32x2 d = add2(pack2(rd[r].f32(i), rd[r].f32(i + 1)), bias);
+            if (p.softplus) d = softplus2(d);
+            *reinterpret_cast<ulonglong2*>(dst0 + r * TS * K::DROW + 2 * i) =
+                make_ulonglong2(d, mul2(d, pack2(rx[r].f32(i), rx[r].f32(i + 1))));
           }
-          if (!live) d0 = d1 = 0.f;  // behind the end: decay 1, and x is 0: input 0
-          *reinterpret_cast<float4*>(dst + 2 * i) = make_float4(d0, d1, d0 * rx.f32(i), d1 * rx.f32(i + 1));
         }
       }
       meet();
-      if (t0 + TT < t1) fetch(t0 + TT, stage ^ 1, emit);
-      const int live = (int)(sp.len - t0 < TT ? sp.len - t0 : TT);
-      // operands of the next U tokens are read before this U are computed, and
-      // the U partial sums stored after it: a store between would hold back
-      // every later read
-      constexpr int U = NP * NS <= 4 ? 2 : 1;
-      Raw<T, NS> nb[U], nc[U];
-      ulonglong2 nd[U][NP];
-      auto operands = [&](int t0) {
+      if (t0 + TT < t1) fetch(stage ^ 1, emit);
+      const int live = min_i(len - t0, TT);
+      // Software pipeline: while token t is accumulated, the decays of t + 1 are
+      // computed (the exponentials' pipe is the scarce one) and the operands of
+      // t + 2 read. Reads past the tile wrap around; nothing uses them.
+      const T* bp0 = sB + lane * NS;
+      const T* cp0 = sC + lane * NS;
+      ulonglong2 nd[NP];       // (delta, delta x) of t + 1
+      f32x2 dx[NP], e[NP][NS]; // delta x and decays of t
+      Raw<T, NS> nb, nc;       // B, C of t
+      auto read_d = [&](int t, ulonglong2 (&d)[NP]) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int t = t0 + u;
-          move<T, NS>(&nb[u], reinterpret_cast<const Raw<T, NS>*>(sB + t * N + lane * NS));
-          if (emit) move<T, NS>(&nc[u], reinterpret_cast<const Raw<T, NS>*>(sC + t * N + lane * NS));
-#pragma unroll
-          for (int j = 0; j < NP; ++j)
-            nd[u][j] = *reinterpret_cast<const ulonglong2*>(sD + t * K::DROW + padded(4 * (ch + j * CBP)));
-        }
+        for (int j = 0; j < NP; ++j)
+          d[j] = *reinterpret_cast<const ulonglong2*>(dp0 + t * K::DROW + padded(4 * j * CBP));
       };
-      operands(0);
-#pragma unroll(4 / U)
-      for (int tb = 0; tb < live; tb += U) {
-        Raw<T, NS> kb[U], kc[U];
-        ulonglong2 kd[U][NP];
-        f32x2 y[U][NP];
+      auto read_bc = [&](int t, Raw<T, NS>& b, Raw<T, NS>& c) {
+        move<T, NS>(&b, reinterpret_cast<const Raw<T, NS>*>(bp0 + t * N));
+        if (emit) move<T, NS>(&c, reinterpret_cast<const Raw<T, NS>*>(cp0 + t * N));
+      };
+      read_d(0, nd);
+      read_bc(0, nb, nc);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          kb[u] = nb[u];
-          if (emit) kc[u] = nc[u];
+      for (int j = 0; j < NP; ++j) {
+        dx[j] = nd[j].y;
+        if (!emit) steps[j] = add2(steps[j], nd[j].x);
 #pragma unroll
-          for (int j = 0; j < NP; ++j) kd[u][j] = nd[u][j];
+        for (int i = 0; i < NS; ++i) {
+          const float2 v = unpack2(mul2(a[j][i], nd[j].x));
+          e[j][i] = pack2(ex2(v.x), ex2(v.y));
         }
-        if (tb + U < TT) operands(tb + U);
+      }
+      read_d(1, nd);
+#pragma unroll 4
+      for (int t = 0; t < live; ++t) {
+        const Raw<T, NS> kb = nb, kc = nc;
+        ulonglong2 kd[NP];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+        for (int j = 0; j < NP; ++j) kd[j] = nd[j];
+        read_bc((t + 1) % TT, nb, nc);
+        read_d((t + 2) % TT, nd);
+        f32x2 y[NP];
 #pragma unroll
-          for (int i = 0; i < NS; ++i) {
-            const f32x2 b2 = pack2(kb[u].f32(i), kb[u].f32(i));
-            const f32x2 c2 = emit ? pack2(kc[u].f32(i), kc[u].f32(i)) : 0;
+        for (int i = 0; i < NS; ++i) {
+          const f32x2 b2 = pack2(kb.f32(i), kb.f32(i));
+          const f32x2 c2 = emit ? pack2(kc.f32(i), kc.f32(i)) : 0;
 #pragma unroll
-            for (int j = 0; j < NP; ++j) {
-              const float2 e = unpack2(mul2(a[j][i], kd[u][j].x));
-              h[j][i] = fma2(pack2(ex2(e.x), ex2(e.y)), h[j][i], mul2(kd[u][j].y, b2));
-              if (emit) y[u][j] = i ? fma2(h[j][i], c2, y[u][j]) : mul2(h[j][i], c2);
-            }
-          }
-          if (!emit) {
-#pragma unroll
-            for (int j = 0; j < NP; ++j) steps[j] = add2(steps[j], kd[u][j].x);
+          for (int j = 0; j < NP; ++j) {
+            const float2 v = unpack2(mul2(a[j][i], kd[j].x));
+            h[j][i] = fma2(e[j][i], h[j][i], mul2(dx[j], b2));
+            e[j][i] = pack2(ex2(v.x), ex2(v.y));
+            if (emit) y[j] = i ? fma2(h[j][i], c2, y[j]) : mul2(h[j][i], c2);
           }
         }
-        if (emit) {
 #pragma unroll
-          for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int j = 0; j < NP; ++j)
-              *reinterpret_cast<f32x2*>(sY + (tb + u) * K::YROW + padded(2 * j * NT) + padded(2 * tid)) = y[u][j];
+        for (int j = 0; j < NP; ++j) {
+          dx[j] = kd[j].y;
+          if (emit)
+            *reinterpret_cast<f32x2*>(y0 + t * K::YROW + padded(2 * j * NT)) = y[j];
+          else if (t + 1 < live)
+            steps[j] = add2(steps[j], kd[j].x);
         }
       }
       meet();
       if (!emit) continue;
+      Raw<T, VE> rx[RV], rz[RV], ry[RV];
 #pragma unroll
       for (int r = 0; r < RV; ++r) {
-        const int t = te + r * TS;
-        if (t0 + t >= sp.len || nv <= 0) continue;
-        const float* src = sY + t * K::YROW + padded(ce * L);
-        Raw<T, VE> rx, rz, out;
-        move<T, VE>(&rx, reinterpret_cast<const Raw<T, VE>*>(sX + t * CB + ce));
-        if (zp) move<T, VE>(&rz, reinterpret_cast<const Raw<T, VE>*>(sX + 2 * TT * CB + t * CB + ce));
+        move<T, VE>(&rx[r], reinterpret_cast<const Raw<T, VE>*>(own + r * TS * CB));
+        if (zp) move<T, VE>(&rz[r], reinterpret_cast<const Raw<T, VE>*>(own + 2 * TT * CB + r * TS * CB));
+      }
 #pragma unroll
-        for (int i = 0; i < VE; i += 2) {
-          const float2 skip = *reinterpret_cast<const float2*>(sP + CB + ce + i);
-          float2 y = make_float2(0.f, 0.f);
+      for (int i = 0; i < VE; i += 2) {
+        const f32x2 skip = *reinterpret_cast<const f32x2*>(sp0 + CB + i);
 #pragma unroll
-          for (int j = 0; j < L; ++j) {
-            const float2 f = *reinterpret_cast<const float2*>(src + padded(i * L + 2 * j));
-            y.x += f.x;
-            y.y += f.y;
+        for (int r = 0; r < RV; ++r) {
+          const float* src = src0 + r * TS * K::YROW;
+          f32x2 sum = 0;
+          if constexpr (L >= 2) {
+#pragma unroll
+            for (int j = 0; j < L; j += 2) {
+              const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(src + padded(i * L + 2 * j));
+              sum = j ? add2(sum, add2(f.x, f.y)) : add2(f.x, f.y);
+            }
+          } else {
+            sum = *reinterpret_cast<const f32x2*>(src + padded(i));
           }
-          y.x = fmaf(skip.x, rx.f32(i), y.x);
-          y.y = fmaf(skip.y, rx.f32(i + 1), y.y);
+          float2 y = unpack2(fma2(skip, pack2(rx[r].f32(i), rx[r].f32(i + 1)), sum));
           if (zp) {
-            y.x *= silu<sizeof(T) == 4>(rz.f32(i));
-            y.y *= silu<sizeof(T) == 4>(rz.f32(i + 1));
+            y.x *= silu<sizeof(T) == 4>(rz[r].f32(i));
+            y.y *= silu<sizeof(T) == 4>(rz[r].f32(i + 1));
           }
-          out.set(i, y.x);
-          out.set(i + 1, y.y);
+          ry[r].set2(i, y.x, y.y);
         }
-        T* dst = op + (t0 + t) * p.D;
+      }
+#pragma unroll
+      for (int r = 0; r < RV; ++r) {
+        if (te + r * TS >= live) continue;
+        T* dst = out + (int64_t)(r * TS) * p.D;
         if (q.vec_x) {
-          move<T, VE>(reinterpret_cast<Raw<T, VE>*>(dst), &out);
+          if (nv > 0) move<T, VE>(reinterpret_cast<Raw<T, VE>*>(dst), &ry[r]);
         } else {
 #pragma unroll
           for (int i = 0; i < VE; ++i)
-            if (i < nv) dst[i] = from_f32<T>(out.f32(i));
+            if (i < nv) dst[i] = from_f32<T>(ry[r].f32(i));
         }
       }
+      out += TT * (int64_t)p.D;
     }
   };
 
   if constexpr (CLUSTER) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
-    const int64_t tiles = (sp.len + TT - 1) / TT, each = (tiles + q.parts - 1) / q.parts * TT;
-    const int64_t b0 = part * each < sp.len ? part * each : sp.len;
-    const int64_t b1 = b0 + each < sp.len ? b0 + each : sp.len;
+    const int64_t each = ((int64_t)(len + TT - 1) / TT + q.parts - 1) / q.parts * TT;
+    const int b0 = (int)(part * each < len ? part * each : len);
+    const int b1 = (int)(b0 + each < len ? b0 + each : len);
     f32x2 start[NP][NS];
 #pragma unroll
     for (int j = 0; j < NP; ++j)
@@ -547,7 +631,7 @@ __global__ void __launch_bounds__(NT) scan_tiles_kernel(TileArgs q) {
     run(b0, b1, true);
     if (part + 1 < q.parts) return;
   } else {
-    run(0, sp.len, true);
+    run(0, len, true);
   }
   if (!p.h_out) return;
 #pragma unroll
@@ -587,10 +671,10 @@ int allow(int bytes, bool big_cluster) {
   return WKVM_OK;
 }
 
-template <typename T, int N, int NP, int NS, int NT, int TT>
-int launch_tiles(const ScanArgs& s, cudaStream_t st) {
+template <typename T, int N, int NP, int NS, int NT, int TT, bool CLUSTER>
+int launch_tiles(const ScanArgs& s, int parts, cudaStream_t st) {
   using K = Tile<T, N, NP, NS, NT, TT>;
-  TileArgs q{s, 0, 1, false, false, false};
+  TileArgs q{s, 0, parts, false, false, false};
   const int per_group = s.D / s.G;
   q.cblocks = (per_group + K::CB - 1) / K::CB;
   const int64_t jobs = (int64_t)s.seqs.nseq * q.cblocks * s.G;
@@ -601,33 +685,21 @@ int launch_tiles(const ScanArgs& s, cudaStream_t st) {
             (!s.z.p || (even(s.z, K::VE) && aligned_to(s.z.p, ax)));
   q.vec_b = even(s.B, K::VB) && even(s.C, K::VB) && aligned_to(s.B.p, ab) && aligned_to(s.C.p, ab);
   q.longest_first = s.seqs.cu && s.seqs.nseq > 1 && s.seqs.nseq <= 256;
-  // Split sequences in time when whole ones give the SMs too few warps: a
-  // split pays twice for the exponentials, so two parts gain nothing.
-  const int64_t tokens = s.seqs.cu ? s.seqs.T / s.seqs.nseq : s.seqs.T;
-  int parts = 1;
-  while (parts < 16 && jobs * parts * 2 <= 2048 && tokens >= (int64_t)parts * 8 * TT) parts *= 2;
-  if (parts < 4) parts = 1;
-  q.parts = parts;
   if (jobs * parts > INT32_MAX) return WKVM_ERR_SHAPE;
-  if (parts == 1) {
-    constexpr auto kern = scan_tiles_kernel<T, N, NP, NS, NT, TT, false>;
-    if (int rc = allow<kern>(K::bytes(false), false)) return rc;
-    kern<<<(unsigned)jobs, NT, K::bytes(false), st>>>(q);
-    return cudaGetLastError() == cudaSuccess ? WKVM_OK : WKVM_ERR_CUDA;
-  }
-  constexpr auto kern = scan_tiles_kernel<T, N, NP, NS, NT, TT, true>;
-  if (int rc = allow<kern>(K::bytes(true), true)) return rc;
+  constexpr auto kern = scan_tiles_kernel<T, N, NP, NS, NT, TT, CLUSTER>;
+  constexpr int bytes = K::bytes(CLUSTER);
+  if (int rc = allow<kern>(bytes, CLUSTER)) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(jobs * parts));
   cfg.blockDim = dim3(NT);
-  cfg.dynamicSmemBytes = K::bytes(true);
+  cfg.dynamicSmemBytes = bytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)parts;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = CLUSTER ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kern, q) == cudaSuccess ? WKVM_OK : WKVM_ERR_CUDA;
 }
 
@@ -635,8 +707,21 @@ template <typename T, int N>
 int launch_scan_n(const ScanArgs& a, cudaStream_t st) {
   // a few tokens of every row: the state's traffic decides, so the row kernel
   if (!a.seqs.cu && a.seqs.T <= 8) return launch_rows<T, N>(a, st);
-  constexpr int NS = N == 128 ? 8 : 4;
-  return launch_tiles<T, N, 1, NS, 32, 16>(a, st);
+  // Warps that four states (two channels) a thread give, of 592 schedulers.
+  // Few: sequences are split in time over clusters (one of 8192 x 4096: 469 us
+  // against 650 whole). A split pays twice for the exponentials, so it takes
+  // four parts at least and room for them. Sequences of unequal length, or not
+  // enough rows for two waves: two states a thread, twice the warps (sixteen
+  // packed prompts of 32768 x 2048 in all: 630 us against 790). Else four (16
+  // equal ones of 2048: 500 us against 635).
+  constexpr int kFine = N == 128 ? 4 : 2, kWide = 2 * kFine;
+  const int64_t warps = (int64_t)a.seqs.nseq * a.D * N / (kWide * 2 * 32);
+  const int64_t tokens = a.seqs.cu ? a.seqs.T / a.seqs.nseq : a.seqs.T;
+  int parts = 1;
+  while (parts < 16 && warps * parts * 2 <= 2048 && tokens >= parts * 8 * 16) parts *= 2;
+  if (warps <= 256 && parts >= 4) return launch_tiles<T, N, 1, kWide, 64, 16, true>(a, parts, st);
+  if (a.seqs.cu || warps < 2048) return launch_tiles<T, N, 1, kFine, 64, 32, false>(a, 1, st);
+  return launch_tiles<T, N, 1, kWide, 64, 16, false>(a, 1, st);
 }
 
 template <typename T>

@@ -54,15 +54,6 @@ __device__ __forceinline__ bool state_row(const int32_t* ids, int64_t num_slots,
   return !ids || (*row >= 0 && *row < num_slots);
 }
 
-// x * sigmoid(x). EXACT: the 32-bit functions (fp32 outputs); otherwise the
-// hardware approximations, whose 2^-21 is far below a 16-bit output's
-// rounding.
-template <bool EXACT>
-__device__ __forceinline__ float silu(float x) {
-  if constexpr (EXACT) return x / (1.0f + expf(-x));
-  return __fdividef(x, 1.0f + __expf(-x));
-}
-
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -71,21 +62,36 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// x * sigmoid(x). EXACT: the 32-bit functions (fp32 outputs); otherwise the
+// hardware approximations, whose 2^-21 is far below a 16-bit output's
+// rounding.
+template <bool EXACT>
+__device__ __forceinline__ float silu(float x) {
+  if constexpr (EXACT) return x / (1.0f + expf(-x));
+  return x * rcp(1.0f + ex2(-kLog2e * x));
+}
+
 // log(1 + e^x) to about 2^-21 relative, small values too: max(x, 0) +
 // log1p(e^-|x|). log1p(e) on [0, 1] is e times a polynomial of degree 8,
 // minimax in the relative error (Remez exchange, 3e-8; 2^-22.2 with fp32
 // rounding). The step scales every exponent of the scan, so it keeps fp32.
+__host__ __device__ constexpr float log1p_coeff(int i) {
+  return i == 0 ? 0.99999994f : i == 1 ? -0.49999493f : i == 2 ? 0.33319098f : i == 3 ? -0.24842982f
+       : i == 4 ? 0.19106007f : i == 5 ? -0.13663246f : i == 6 ? 0.078225955f : i == 7 ? -0.029505240f
+       : 0.0052326931f;
+}
+
 __device__ __forceinline__ float softplus(float x) {
   const float e = ex2(-kLog2e * fabsf(x));
-  float p = 0.0052326931f;
-  p = fmaf(p, e, -0.029505240f);
-  p = fmaf(p, e, 0.078225955f);
-  p = fmaf(p, e, -0.13663246f);
-  p = fmaf(p, e, 0.19106007f);
-  p = fmaf(p, e, -0.24842982f);
-  p = fmaf(p, e, 0.33319098f);
-  p = fmaf(p, e, -0.49999493f);
-  p = fmaf(p, e, 0.99999994f);
+  float p = log1p_coeff(8);
+#pragma unroll
+  for (int i = 7; i >= 0; --i) p = fmaf(p, e, log1p_coeff(i));
   return fmaf(p, e, fmaxf(x, 0.0f));
 }
 
