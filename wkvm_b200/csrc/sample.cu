@@ -21,13 +21,13 @@
 // moves a mass by V 2^-(s+1) at most, 2^-31 of the largest weight there.
 //
 // All three filters keep a prefix of the descending order, so what is kept is
-// one logit and a bound on the ids that equal it. A row's CTAs (one when there
-// are many rows, a cluster when there are few) find that bound by histograms
+// one logit and a bound on the ids that equal it. A row's CTAs (a cluster for
+// large vocabularies and few rows) find that bound by histograms
 // of counts (top-k) or masses (top-p) over the logits above a lower bound,
 // then finish on a sorted list of at most kCap candidates in one CTA. Only a
 // larger set is narrowed by further histograms and drawn from by a pass over
-// the whole row. HBM is read once: later passes find short slices in shared
-// memory and long ones in L2 (148 rows of 65,536 fp32 logits are 39 MB).
+// the whole row. HBM is read once: later passes find the slice in shared
+// memory, or, in vocabularies too long for eight CTAs', in L2.
 #include <cooperative_groups.h>
 #include <float.h>
 
@@ -892,10 +892,13 @@ extern "C" int wkvm_sample_tokens(const void* logits, int64_t row_stride, const 
   if (V > WKVM_SAMPLE_MAX_VOCAB) return WKVM_ERR_SHAPE;
   if (B == 0) return WKVM_OK;
   if (!logits || !u || !tokens || !logprobs) return WKVM_ERR_INVALID_ARG;
-  // Rows alone fill the 148 SMs from 128 on; fewer are split over a cluster
-  // as long as a CTA keeps two logits a thread.
+  // Slices of 16,384 fit shared memory and spread the rows that need several
+  // passes (256 mixed rows of 65,536: 98 us over four CTAs each, 158 whole, 117
+  // over eight). Few rows take more CTAs (one: 34 us over eight, 45 over four).
   int ctas = 1;
-  while (ctas < wkvm::kMaxCtas && (int64_t)B * ctas < 128 && V >= ctas * 2048) ctas *= 2;
+  while (ctas < wkvm::kMaxCtas &&
+         (V > ctas * wkvm::kSmemSlice || ((int64_t)B * ctas <= 256 && V >= ctas * 2048)))
+    ctas *= 2;
   if ((int64_t)B * ctas > INT32_MAX) return WKVM_ERR_SHAPE;
   const int64_t es = dtype == WKVM_DTYPE_F32 ? 4 : 2;
   const int slice = ((V + ctas - 1) / ctas + wkvm::kNT - 1) / wkvm::kNT * wkvm::kNT;
