@@ -36,11 +36,14 @@ struct ScanArgs {
 };
 
 // ---------------------------------------------------------------------------
-// Row kernel: the state streams through registers once, T tokens applied in
-// order. For single tokens it moves 8 N bytes of state per channel against
-// some 8 bytes of activations, so HBM bounds it. Four states (16 bytes) a
-// thread: a warp's accesses are contiguous, and y takes a butterfly over the
-// N/4 lanes of a channel.
+// Row kernel: the states of a block of channels of one sequence stream through
+// registers once, T tokens applied in order. A single token moves 8 N bytes of
+// state per channel against some 8 bytes of activations, so HBM bounds it.
+// Four states (16 bytes) of J channels a thread: a warp's accesses are
+// contiguous, J loads of state are in flight, and a thread's B and C serve its
+// J channels. What is per channel (step, gate) is computed once, by one thread,
+// and read from shared memory by the N/4 lanes that need it. Blocks of the same
+// channels are neighbours, so A comes from L1 and L2.
 // ---------------------------------------------------------------------------
 constexpr int kRowThreads = 128;
 
@@ -48,63 +51,86 @@ constexpr int kRowThreads = 128;
 // state even where A is -inf.
 __device__ __forceinline__ float scaled(float a) { return fmaxf(a * kLog2e, -FLT_MAX); }
 
-template <typename T, int N>
+template <typename T, int N, int J>
 __global__ void __launch_bounds__(kRowThreads) scan_rows_kernel(ScanArgs p) {
   constexpr int LPC = N / 4;  // lanes of a channel
-  constexpr int CPB = kRowThreads / LPC;
-  const int cblocks = (p.D + CPB - 1) / CPB;
-  const int n = blockIdx.x / cblocks;
-  const int lane = threadIdx.x % LPC;
-  const int d = (blockIdx.x - n * cblocks) * CPB + threadIdx.x / LPC;
+  constexpr int STEP = kRowThreads / LPC, CPB = STEP * J;
+  __shared__ float4 s_ch[CPB];  // delta, delta x, D x, gate
+  __shared__ float s_y[CPB];
+  const int n = blockIdx.x % p.seqs.nseq, c0 = blockIdx.x / p.seqs.nseq * CPB;
+  const int tid = threadIdx.x, lane = tid % LPC, ch = tid / LPC;
   int64_t row;
-  const SeqSpan sp = seq_span(p.seqs, n);
   if (!state_row(p.ids, p.num_slots, n, &row)) {
-    if (threadIdx.x == 0) report(p.status, WKVM_ERR_SLOT_RANGE);
+    if (tid == 0) report(p.status, WKVM_ERR_SLOT_RANGE);
     return;
   }
-  if (!sp.ok) {
-    if (threadIdx.x == 0) report(p.status, WKVM_ERR_INVALID_ARG);
-    return;
-  }
-  const bool on = d < p.D;  // the butterfly needs every lane
-  const int dc = on ? d : p.D - 1;
-  const int64_t hoff = (row * p.D + dc) * N + lane * 4;
-  float4 h = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (p.h_in) h = ld_stream_f4(p.h_in + hoff);
-  float4 a = *reinterpret_cast<const float4*>(p.A + (int64_t)dc * N + lane * 4);
-  a.x = scaled(a.x); a.y = scaled(a.y); a.z = scaled(a.z); a.w = scaled(a.w);
-  const float bias = p.bias ? p.bias[dc] : 0.f, skip = p.skip ? p.skip[dc] : 0.f;
-  const int g = dc / (p.D / p.G);
-  const T* xp = static_cast<const T*>(p.x.p) + act_row(p.seqs, p.x, n, sp.bos) + dc;
-  const T* dp = static_cast<const T*>(p.dt.p) + act_row(p.seqs, p.dt, n, sp.bos) + dc;
-  const T* bp = static_cast<const T*>(p.B.p) + act_row(p.seqs, p.B, n, sp.bos) + g * N + lane * 4;
-  const T* cp = static_cast<const T*>(p.C.p) + act_row(p.seqs, p.C, n, sp.bos) + g * N + lane * 4;
-  const T* zp = p.z.p ? static_cast<const T*>(p.z.p) + act_row(p.seqs, p.z, n, sp.bos) + dc : nullptr;
-  T* op = static_cast<T*>(p.o) + sp.bos * p.D + dc;
-  for (int64_t t = 0; t < sp.len; ++t) {
-    const float x = to_f32(xp[t * p.x.ts]);
-    float delta = to_f32(dp[t * p.dt.ts]) + bias;
-    if (p.softplus) delta = softplus(delta);
-    float bv[4], cv[4];
+  const int live = p.D - c0 < CPB ? p.D - c0 : CPB;  // channels of this block
+  const int64_t hoff = (row * p.D + c0 + ch) * N + lane * 4;
+  const float* ap = p.A + (int64_t)(c0 + ch) * N + lane * 4;
+  float4 h[J];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      bv[i] = to_f32(bp[t * p.B.ts + i]);
-      cv[i] = to_f32(cp[t * p.C.ts + i]);
+  for (int j = 0; j < J; ++j) {
+    h[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (p.h_in && ch + j * STEP < live) h[j] = ld_stream_f4(p.h_in + hoff + j * STEP * N);
+  }
+  const int per_group = p.D / p.G;
+  const T* xp = static_cast<const T*>(p.x.p) + n * p.x.bs + c0;
+  const T* dp = static_cast<const T*>(p.dt.p) + n * p.dt.bs + c0;
+  const T* zp = static_cast<const T*>(p.z.p) + n * p.z.bs + c0;
+  const T* bp = static_cast<const T*>(p.B.p) + n * p.B.bs + lane * 4;
+  const T* cp = static_cast<const T*>(p.C.p) + n * p.C.bs + lane * 4;
+  T* op = static_cast<T*>(p.o) + (int64_t)n * p.seqs.T * p.D + c0;
+  const bool one_group = c0 / per_group == (c0 + live - 1) / per_group;
+  for (int t = 0; t < p.seqs.T; ++t) {
+    for (int c = tid; c < live; c += kRowThreads) {
+      const float x = to_f32(xp[t * p.x.ts + c]);
+      float delta = to_f32(dp[t * p.dt.ts + c]) + (p.bias ? p.bias[c0 + c] : 0.f);
+      if (p.softplus) delta = softplus(delta);
+      const float gate = p.z.p ? silu<true>(to_f32(zp[t * p.z.ts + c])) : 1.f;
+      s_ch[c] = make_float4(delta, delta * x, p.skip ? p.skip[c0 + c] * x : 0.f, gate);
     }
-    const float z = zp ? to_f32(zp[t * p.z.ts]) : 0.f;
-    const float dx = delta * x;
-    h.x = fmaf(ex2(delta * a.x), h.x, dx * bv[0]);
-    h.y = fmaf(ex2(delta * a.y), h.y, dx * bv[1]);
-    h.z = fmaf(ex2(delta * a.z), h.z, dx * bv[2]);
-    h.w = fmaf(ex2(delta * a.w), h.w, dx * bv[3]);
-    float y = fmaf(h.x, cv[0], h.y * cv[1]) + fmaf(h.z, cv[2], h.w * cv[3]);
+    __syncthreads();
+    float bv[4], cv[4];
+    int g = c0 / per_group;
+    auto read_bc = [&] {
 #pragma unroll
-    for (int off = LPC / 2; off > 0; off >>= 1) y += __shfl_xor_sync(0xffffffffu, y, off);
-    y = fmaf(skip, x, y);
-    if (zp) y *= silu<true>(z);
-    if (on && lane == 0) op[t * p.D] = from_f32<T>(y);
+      for (int i = 0; i < 4; ++i) {
+        bv[i] = to_f32(bp[t * p.B.ts + g * N + i]);
+        cv[i] = to_f32(cp[t * p.C.ts + g * N + i]);
+      }
+    };
+    if (one_group) read_bc();
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int c = ch + j * STEP;
+      float y = 0.f;
+      if (c < live) {
+        if (!one_group) {
+          g = (c0 + c) / per_group;
+          read_bc();
+        }
+        const float2 s = *reinterpret_cast<const float2*>(&s_ch[c]);
+        const float4 a = *reinterpret_cast<const float4*>(ap + j * STEP * N);
+        h[j].x = fmaf(ex2(s.x * scaled(a.x)), h[j].x, s.y * bv[0]);
+        h[j].y = fmaf(ex2(s.x * scaled(a.y)), h[j].y, s.y * bv[1]);
+        h[j].z = fmaf(ex2(s.x * scaled(a.z)), h[j].z, s.y * bv[2]);
+        h[j].w = fmaf(ex2(s.x * scaled(a.w)), h[j].w, s.y * bv[3]);
+        y = fmaf(h[j].x, cv[0], h[j].y * cv[1]) + fmaf(h[j].z, cv[2], h[j].w * cv[3]);
+      }
+#pragma unroll
+      for (int off = LPC / 2; off > 0; off >>= 1) y += __shfl_xor_sync(0xffffffffu, y, off);
+      if (lane == 0) s_y[c] = y;
+    }
+    __syncthreads();
+    for (int c = tid; c < live; c += kRowThreads) {
+      const float2 s = reinterpret_cast<const float2*>(&s_ch[c])[1];
+      op[(int64_t)t * p.D + c] = from_f32<T>((s_y[c] + s.x) * s.y);
+    }
   }
-  if (on && p.h_out) st_stream_f4(p.h_out + hoff, h);
+  if (!p.h_out) return;
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+    if (ch + j * STEP < live) st_stream_f4(p.h_out + hoff + j * STEP * N, h[j]);
 }
 
 // ---------------------------------------------------------------------------
@@ -127,36 +153,6 @@ __global__ void __launch_bounds__(kRowThreads) scan_rows_kernel(ScanArgs p) {
 // the part's whole decay, A being constant), then takes the parts before it
 // from its peers' shared memory and runs its part again from its true start.
 // ---------------------------------------------------------------------------
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pack2(float x, float y) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ float2 unpack2(f32x2 v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-
-// V elements as they lie in memory, held as words: elements of 16 bits kept
-// apart would be taken apart, and so waited for, right after the load.
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
 // softplus() of two
 __device__ __forceinline__ f32x2 softplus2(f32x2 x) {
   const float2 v = unpack2(x);
@@ -165,56 +161,6 @@ __device__ __forceinline__ f32x2 softplus2(f32x2 x) {
 #pragma unroll
   for (int i = 7; i >= 0; --i) q = fma2(q, e, pack2(log1p_coeff(i), log1p_coeff(i)));
   return fma2(q, e, pack2(fmaxf(v.x, 0.0f), fmaxf(v.y, 0.0f)));
-}
-
-template <typename T, int V>
-struct Raw {
-  static constexpr int kBytes = sizeof(T) * V, kWords = (kBytes + 3) / 4;
-  uint32_t w[kWords];
-  __device__ __forceinline__ float f32(int i) const {
-    if constexpr (sizeof(T) == 4) {
-      return __uint_as_float(w[i]);
-    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-      // byte permutes: the compiler's shifts by multiplication would crowd the
-      // fp32 pipe
-      uint32_t x;
-      if (i % 2)
-        asm("prmt.b32 %0, %1, 0, 0x3244;" : "=r"(x) : "r"(w[i / 2]));
-      else
-        asm("prmt.b32 %0, %1, 0, 0x1044;" : "=r"(x) : "r"(w[i / 2]));
-      return __uint_as_float(x);
-    } else {
-      const uint16_t h = (uint16_t)(w[i / 2] >> (16 * (i % 2)));
-      return to_f32(*reinterpret_cast<const T*>(&h));
-    }
-  }
-  __device__ __forceinline__ void set2(int i, float x, float y) {  // elements i and i + 1, i even
-    if constexpr (sizeof(T) == 4) {
-      w[i] = __float_as_uint(x);
-      w[i + 1] = __float_as_uint(y);
-    } else if constexpr (std::is_same<T, __half>::value) {
-      const __half2 h = __floats2half2_rn(x, y);
-      w[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
-    } else {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-      w[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-  }
-};
-
-template <typename T, int V>
-__device__ __forceinline__ void move(Raw<T, V>* dst, const Raw<T, V>* src) {  // one access each way
-  constexpr int B = Raw<T, V>::kBytes;
-  if constexpr (B >= 16) {
-#pragma unroll
-    for (int i = 0; i < B / 16; ++i) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
-  } else if constexpr (B == 8) {
-    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(src);
-  } else if constexpr (B == 4) {
-    *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
-  } else {
-    *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(src);
-  }
 }
 
 // V elements at p, of which the first `n` exist (the others read as zero).
@@ -647,12 +593,12 @@ __global__ void __launch_bounds__(NT) scan_tiles_kernel(TileArgs q) {
   }
 }
 
-template <typename T, int N>
+template <typename T, int N, int J>
 int launch_rows(const ScanArgs& a, cudaStream_t st) {
-  constexpr int CPB = kRowThreads / (N / 4);
+  constexpr int CPB = kRowThreads / (N / 4) * J;
   const int64_t blocks = (int64_t)a.seqs.nseq * ((a.D + CPB - 1) / CPB);
   if (blocks > INT32_MAX) return WKVM_ERR_SHAPE;
-  scan_rows_kernel<T, N><<<(unsigned)blocks, kRowThreads, 0, st>>>(a);
+  scan_rows_kernel<T, N, J><<<(unsigned)blocks, kRowThreads, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? WKVM_OK : WKVM_ERR_CUDA;
 }
 
@@ -706,7 +652,11 @@ int launch_tiles(const ScanArgs& s, int parts, cudaStream_t st) {
 template <typename T, int N>
 int launch_scan_n(const ScanArgs& a, cudaStream_t st) {
   // a few tokens of every row: the state's traffic decides, so the row kernel
-  if (!a.seqs.cu && a.seqs.T <= 8) return launch_rows<T, N>(a, st);
+  if (!a.seqs.cu && a.seqs.T <= 8) {
+    // eight channels a thread once that still gives every SM its threads
+    if ((int64_t)a.seqs.nseq * a.D * N / 4 >= 148 * 1024 * 8) return launch_rows<T, N, 8>(a, st);
+    return launch_rows<T, N, 1>(a, st);
+  }
   // Warps that four states (two channels) a thread give, of 592 schedulers.
   // Few: sequences are split in time over clusters (one of 8192 x 4096: 469 us
   // against 650 whole). A split pays twice for the exponentials, so it takes

@@ -8,21 +8,22 @@
 // convolution of selective state space layers and of gated-delta-rule layers.
 //
 // Streaming: every input is read once, every output written once, 2 W FLOPs
-// each, so HBM bounds it. One thread owns 16 bytes of channels and keeps the
-// window in registers.
+// each, so HBM bounds it. One thread owns a few neighbouring channels and keeps
+// their weights and window in registers, two channels to a pair.
 //
-// The launch has two kinds of blocks. Sequence blocks compute the first
-// W - 1 outputs of a sequence (those that need the state row) and then write
-// its new row; nobody else touches a state row, so the update in place needs
-// no second launch and no order between blocks. Tile blocks compute every
-// other output from the inputs alone, kTile tokens each, wherever sequences
-// begin and end inside the tile.
+// A sequence's first W - 1 outputs need its state row, which the call also
+// replaces. Sequence blocks do both, so nobody else touches a state row: the
+// update in place needs no second launch and no order between blocks. Every
+// other output needs inputs alone and belongs to a tile block, kTile tokens
+// each, wherever sequences begin and end inside the tile. Short rows (a decode
+// step) run in sequence blocks alone.
 #include "ssm_common.cuh"
 
 namespace wkvm {
 namespace {
 
-constexpr int kTile = 16;     // tokens of a tile block: the window's re-read is (W-1)/16
+constexpr int kTile = 32;     // tokens of a tile block: the window's re-read is (W-1)/32
+constexpr int kFly = 8;       // inputs of a tile in flight a thread
 constexpr int kThreads = 128;
 
 struct ConvArgs {
@@ -41,62 +42,101 @@ struct ConvArgs {
   int* status;
 };
 
-template <typename T, int V> struct alignas(sizeof(T) * V) Vec { T e[V]; };
+// Arithmetic of a lane: two channels in a register pair, or one.
+template <int V> using Pair = std::conditional_t<(V > 1), f32x2, float>;
+__device__ __forceinline__ f32x2 fma_(f32x2 a, f32x2 b, f32x2 c) { return fma2(a, b, c); }
+__device__ __forceinline__ float fma_(float a, float b, float c) { return fmaf(a, b, c); }
+
+template <bool EXACT>
+__device__ __forceinline__ float silu_of(float x) { return silu<EXACT>(x); }
+template <bool EXACT>
+__device__ __forceinline__ f32x2 silu_of(f32x2 x) {
+  if constexpr (EXACT) {
+    const float2 v = unpack2(x);
+    return pack2(silu<true>(v.x), silu<true>(v.y));
+  } else {
+    const float2 t = unpack2(mul2(x, pack2(-kLog2e, -kLog2e)));
+    const float2 d = unpack2(add2(pack2(ex2(t.x), ex2(t.y)), pack2(1.f, 1.f)));
+    return mul2(x, pack2(rcp(d.x), rcp(d.y)));
+  }
+}
 
 template <typename T, int V>
-__device__ __forceinline__ void load_vec(const T* p, float (&v)[V]) {
-  const Vec<T, V> u = *reinterpret_cast<const Vec<T, V>*>(p);
+__device__ __forceinline__ void widen(const Raw<T, V>& r, Pair<V> (&v)[(V + 1) / 2]) {
+  if constexpr (V == 1) {
+    v[0] = r.f32(0);
+  } else {
 #pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = to_f32(u.e[i]);
+    for (int i = 0; i < V / 2; ++i) v[i] = pack2(r.f32(2 * i), r.f32(2 * i + 1));
+  }
 }
 template <typename T, int V>
-__device__ __forceinline__ void store_vec(T* p, const float (&v)[V]) {
-  Vec<T, V> u;
-#pragma unroll
-  for (int i = 0; i < V; ++i) u.e[i] = from_f32<T>(v[i]);
-  *reinterpret_cast<Vec<T, V>*>(p) = u;
+__device__ __forceinline__ Raw<T, V> load_raw(const T* p) {
+  Raw<T, V> r;
+  if constexpr (Raw<T, V>::kBytes == 2)
+    r.w[0] = *reinterpret_cast<const uint16_t*>(p);
+  else
+    move<T, V>(&r, reinterpret_cast<const Raw<T, V>*>(p));
+  return r;
 }
 
-template <typename T, int V, int W, bool SILU>
+template <typename T, int V, int W, bool SILU, bool TILES>
 __global__ void __launch_bounds__(kThreads) short_conv_kernel(ConvArgs p) {
+  constexpr int P = (V + 1) / 2;
   const int DV = p.D / V;
   const T* wp = static_cast<const T*>(p.w);
   const T* xp = static_cast<const T*>(p.x.p);
   T* op = static_cast<T*>(p.o);
-  float w[W][V], bias[V], win[W][V];  // win: the window, oldest first
+  Pair<V> w[W][P], bias[P], win[W][P];  // win: the window, oldest first
 
   auto load_weights = [&](int c) {
     const T* src = wp + (int64_t)c * W;  // channel-major: V * W contiguous weights
+    Raw<T, V> r[W];
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-      float t[V];
-      load_vec<T, V>(src + j * V, t);
+    for (int j = 0; j < W; ++j) r[j] = load_raw<T, V>(src + j * V);
+    auto at = [&](int i, int j) { return r[(i * W + j) / V].f32((i * W + j) % V); };  // channel i, tap j
 #pragma unroll
-      for (int i = 0; i < V; ++i) w[(j * V + i) % W][(j * V + i) / W] = t[i];
-    }
+    for (int j = 0; j < W; ++j)
 #pragma unroll
-    for (int i = 0; i < V; ++i) bias[i] = 0.f;
-    if (p.bias) load_vec<T, V>(static_cast<const T*>(p.bias) + c, bias);
+      for (int i = 0; i < P; ++i) {
+        if constexpr (V == 1) w[j][i] = at(0, j);
+        else w[j][i] = pack2(at(2 * i, j), at(2 * i + 1, j));
+      }
+#pragma unroll
+    for (int i = 0; i < P; ++i) bias[i] = 0;
+    if (p.bias) widen<T, V>(load_raw<T, V>(static_cast<const T*>(p.bias) + c), bias);
   };
   auto emit = [&](int64_t token, int c) {
-    float y[V];
+    Pair<V> y[P];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float a = bias[i];
+    for (int i = 0; i < P; ++i) {
+      y[i] = bias[i];
 #pragma unroll
-      for (int j = 0; j < W; ++j) a = fmaf(w[j][i], win[j][i], a);
-      y[i] = SILU ? silu<sizeof(T) == 4>(a) : a;
+      for (int j = 0; j < W; ++j) y[i] = fma_(w[j][i], win[j][i], y[i]);
+      if (SILU) y[i] = silu_of<sizeof(T) == 4>(y[i]);
     }
-    store_vec<T, V>(op + token * p.D + c, y);
+    T* dst = op + token * p.D + c;
+    if constexpr (V == 1) {
+      *dst = from_f32<T>(y[0]);
+    } else {
+      Raw<T, V> out;
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const float2 v = unpack2(y[i]);
+        out.set2(2 * i, v.x, v.y);
+      }
+      move<T, V>(reinterpret_cast<Raw<T, V>*>(dst), &out);
+    }
   };
-  auto shift = [&]() {
+  auto shift = [&](const Raw<T, V>& in) {
 #pragma unroll
     for (int j = 0; j + 1 < W; ++j)
 #pragma unroll
-      for (int i = 0; i < V; ++i) win[j][i] = win[j + 1][i];
+      for (int i = 0; i < P; ++i) win[j][i] = win[j + 1][i];
+    widen<T, V>(in, win[W - 1]);
   };
 
-  if ((int)blockIdx.x < p.seq_blocks) {
+  if (!TILES || (int)blockIdx.x < p.seq_blocks) {
     const int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x;
     if (e >= (int64_t)p.seqs.nseq * DV) return;
     const int n = (int)(e / DV), c = (int)(e - (int64_t)n * DV) * V;
@@ -110,35 +150,46 @@ __global__ void __launch_bounds__(kThreads) short_conv_kernel(ConvArgs p) {
       if (c == 0) report(p.status, WKVM_ERR_INVALID_ARG);
       return;
     }
-    load_weights(c);
     const int64_t srow = row * (W - 1) * p.D + c;
+    const T* xs = xp + act_row(p.seqs, p.x, n, sp.bos) + c;
+    const int64_t head = sp.len < p.head ? sp.len : p.head;
+    Raw<T, V> next;
+    if (head > 0) next = load_raw<T, V>(xs);
 #pragma unroll
     for (int j = 0; j + 1 < W; ++j) {  // win[1..W-1] <- the state row
 #pragma unroll
-      for (int i = 0; i < V; ++i) win[j + 1][i] = 0.f;
-      if (p.s_in) load_vec<T, V>(static_cast<const T*>(p.s_in) + srow + (int64_t)j * p.D, win[j + 1]);
+      for (int i = 0; i < P; ++i) win[j + 1][i] = 0;
+      if (p.s_in) widen<T, V>(load_raw<T, V>(static_cast<const T*>(p.s_in) + srow + (int64_t)j * p.D), win[j + 1]);
     }
-    const T* xs = xp + act_row(p.seqs, p.x, n, sp.bos) + c;
-    const int64_t head = sp.len < p.head ? sp.len : p.head;
+    load_weights(c);
     for (int64_t t = 0; t < head; ++t) {
-      shift();
-      load_vec<T, V>(xs + t * p.x.ts, win[W - 1]);
+      shift(next);
+      if (t + 1 < head) next = load_raw<T, V>(xs + (t + 1) * p.x.ts);
       emit(sp.bos + t, c);
     }
     if (p.s_out) {
-      if (head < sp.len) {  // the last W - 1 inputs lie past the head
+      // the last W - 1 inputs: the sequence's own, ahead of them what it
+      // leaves of the row (read at j + len, so ahead of what is written)
 #pragma unroll
-        for (int j = 0; j + 1 < W; ++j) {
-          const int64_t t = sp.len - (W - 1) + j;  // >= 0: head >= W - 1
-          load_vec<T, V>(xs + t * p.x.ts, win[j + 1]);
-        }
+      for (int j = 0; j + 1 < W; ++j) {
+        const int64_t t = sp.len - (W - 1) + j;
+        T* dst = static_cast<T*>(p.s_out) + srow + (int64_t)j * p.D;
+        Raw<T, V> in;
+#pragma unroll
+        for (int i = 0; i < Raw<T, V>::kWords; ++i) in.w[i] = 0;
+        if (t >= 0)
+          in = load_raw<T, V>(xs + t * p.x.ts);
+        else if (p.s_in)
+          in = load_raw<T, V>(static_cast<const T*>(p.s_in) + srow + (j + sp.len) * p.D);
+        if constexpr (Raw<T, V>::kBytes == 2)
+          *reinterpret_cast<uint16_t*>(dst) = (uint16_t)in.w[0];
+        else
+          move<T, V>(reinterpret_cast<Raw<T, V>*>(dst), &in);
       }
-#pragma unroll
-      for (int j = 0; j + 1 < W; ++j)
-        store_vec<T, V>(static_cast<T*>(p.s_out) + srow + (int64_t)j * p.D, win[j + 1]);
     }
     return;
   }
+  if constexpr (!TILES) return;
 
   // ---- tile block: tokens [t0, t1) of the flattened axis, one channel slice
   const int cblocks = (DV + kThreads - 1) / kThreads;
@@ -162,59 +213,71 @@ __global__ void __launch_bounds__(kThreads) short_conv_kernel(ConvArgs p) {
     if (sp.bos >= t1) break;
     int64_t row;
     if (!sp.ok || !state_row(p.ids, p.num_slots, n, &row)) continue;
-    int64_t t = t0 - sp.bos > p.head ? t0 - sp.bos : p.head;  // tokens of the sequence
+    const int64_t ta = t0 - sp.bos > p.head ? t0 - sp.bos : p.head;  // tokens of the sequence
     const int64_t te = t1 - sp.bos < sp.len ? t1 - sp.bos : sp.len;
-    if (t >= te) continue;
-    const T* xs = xp + act_row(p.seqs, p.x, n, sp.bos) + c;
+    if (ta >= te) continue;
+    const T* xs = xp + act_row(p.seqs, p.x, n, sp.bos) + c + ta * p.x.ts;
+    const int64_t token = sp.bos + ta;
+    const int many = (int)(te - ta);
+    Raw<T, V> in[kFly];
 #pragma unroll
-    for (int j = 0; j + 1 < W; ++j) load_vec<T, V>(xs + (t - (W - 1) + j) * p.x.ts, win[j + 1]);
-    for (; t < te; ++t) {
-      shift();
-      load_vec<T, V>(xs + t * p.x.ts, win[W - 1]);
-      emit(sp.bos + t, c);
+    for (int f = 0; f < kFly; ++f)
+      if (f < many) in[f] = load_raw<T, V>(xs + f * p.x.ts);
+#pragma unroll
+    for (int j = 0; j + 1 < W; ++j) widen<T, V>(load_raw<T, V>(xs + (j - (W - 1)) * p.x.ts), win[j + 1]);
+    for (int t = 0; t < many; t += kFly) {
+#pragma unroll
+      for (int f = 0; f < kFly; ++f) {
+        if (t + f >= many) break;
+        shift(in[f]);
+        if (t + f + kFly < many) in[f] = load_raw<T, V>(xs + (int64_t)(t + f + kFly) * p.x.ts);
+        emit(token + t + f, c);
+      }
     }
   }
 }
 
-template <typename T, int V, int W>
+template <typename T, int V, int W, bool TILES>
 int launch_conv_w(ConvArgs a, bool silu, cudaStream_t st) {
   const int64_t DV = a.D / V;
   const int64_t total = a.seqs.cu ? a.seqs.T : (int64_t)a.seqs.nseq * a.seqs.T;
-  // Short rows (a decode step) run wholly in the sequence blocks: no tile
-  // blocks to launch, and the inputs are read once. Past kTile tokens a
-  // sequence block would be a serial walk, so it keeps the first W - 1 only.
-  const bool tiles = a.seqs.cu ? true : a.seqs.T > kTile;
-  a.head = tiles ? W - 1 : a.seqs.T;
+  a.head = TILES ? W - 1 : a.seqs.T;
   const int64_t sb = ((int64_t)a.seqs.nseq * DV + kThreads - 1) / kThreads;
-  const int64_t tb = tiles ? (total + kTile - 1) / kTile * ((DV + kThreads - 1) / kThreads) : 0;
+  const int64_t tb = TILES ? (total + kTile - 1) / kTile * ((DV + kThreads - 1) / kThreads) : 0;
   if (sb + tb > INT32_MAX) return WKVM_ERR_SHAPE;
   a.seq_blocks = (int32_t)sb;
-  if (silu)
-    short_conv_kernel<T, V, W, true><<<(unsigned)(sb + tb), kThreads, 0, st>>>(a);
-  else
-    short_conv_kernel<T, V, W, false><<<(unsigned)(sb + tb), kThreads, 0, st>>>(a);
+  const auto kern = silu ? short_conv_kernel<T, V, W, true, TILES> : short_conv_kernel<T, V, W, false, TILES>;
+  kern<<<(unsigned)(sb + tb), kThreads, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? WKVM_OK : WKVM_ERR_CUDA;
 }
 
-template <typename T, int V>
+template <typename T, int V, bool TILES>
 int launch_conv_v(const ConvArgs& a, int W, bool silu, cudaStream_t st) {
   switch (W) {
-    case 2: return launch_conv_w<T, V, 2>(a, silu, st);
-    case 3: return launch_conv_w<T, V, 3>(a, silu, st);
-    case 4: return launch_conv_w<T, V, 4>(a, silu, st);
+    case 2: return launch_conv_w<T, V, 2, TILES>(a, silu, st);
+    case 3: return launch_conv_w<T, V, 3, TILES>(a, silu, st);
+    case 4: return launch_conv_w<T, V, 4, TILES>(a, silu, st);
     default: return WKVM_ERR_SHAPE;
   }
 }
 
 template <typename T>
 int launch_conv(const ConvArgs& a, int W, bool silu, cudaStream_t st) {
-  constexpr int V = 16 / sizeof(T);
-  // 16-byte accesses when every row starts on 16 bytes, else one channel a
-  // thread (odd channel counts, views at odd offsets)
-  const bool vec = a.D % V == 0 && a.x.bs % V == 0 && a.x.ts % V == 0 && aligned_to(a.x.p, 16) &&
-                   aligned_to(a.w, 16) && aligned_to(a.bias, 16) && aligned_to(a.o, 16) &&
-                   aligned_to(a.s_in, 16) && aligned_to(a.s_out, 16);
-  return vec ? launch_conv_v<T, V>(a, W, silu, st) : launch_conv_v<T, 1>(a, W, silu, st);
+  // Whole-vector accesses when every row starts on the vector's size, else one
+  // channel a thread (odd channel counts, views at odd offsets). A sequence
+  // block keeps 16 bytes of channels a thread; in a tile, eight 16-bit channels
+  // and their inputs in flight would take 140 registers, so four.
+  constexpr int VS = 16 / sizeof(T), VT = 4;
+  auto fits = [&](int v) {
+    const uintptr_t n = v * sizeof(T);
+    return a.D % v == 0 && a.x.bs % v == 0 && a.x.ts % v == 0 && aligned_to(a.x.p, n) && aligned_to(a.w, n) &&
+           aligned_to(a.bias, n) && aligned_to(a.o, n) && aligned_to(a.s_in, n) && aligned_to(a.s_out, n);
+  };
+  // Past kTile tokens a sequence block would be a serial walk, so it keeps the
+  // first W - 1 only; shorter rows need no tile blocks.
+  if (!a.seqs.cu && a.seqs.T <= kTile)
+    return fits(VS) ? launch_conv_v<T, VS, false>(a, W, silu, st) : launch_conv_v<T, 1, false>(a, W, silu, st);
+  return fits(VT) ? launch_conv_v<T, VT, true>(a, W, silu, st) : launch_conv_v<T, 1, true>(a, W, silu, st);
 }
 
 int run_conv(ConvArgs a, int W, int act, int dtype, cudaStream_t st) {

@@ -2,6 +2,8 @@
 // tokens and its state row lie, and 32-bit activation functions.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace wkvm {
@@ -93,6 +95,87 @@ __device__ __forceinline__ float softplus(float x) {
 #pragma unroll
   for (int i = 7; i >= 0; --i) p = fmaf(p, e, log1p_coeff(i));
   return fmaf(p, e, fmaxf(x, 0.0f));
+}
+
+// Two fp32 in one 64-bit register pair (one instruction for both).
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float x, float y) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// V elements as they lie in memory, held as words: elements of 16 bits kept
+// apart would be taken apart, and so waited for, right after the load.
+template <typename T, int V>
+struct Raw {
+  static constexpr int kBytes = sizeof(T) * V, kWords = (kBytes + 3) / 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ float f32(int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[i]);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      // byte permutes: the compiler's shifts by multiplication would crowd the
+      // fp32 pipe
+      uint32_t x;
+      if (i % 2)
+        asm("prmt.b32 %0, %1, 0, 0x3244;" : "=r"(x) : "r"(w[i / 2]));
+      else
+        asm("prmt.b32 %0, %1, 0, 0x1044;" : "=r"(x) : "r"(w[i / 2]));
+      return __uint_as_float(x);
+    } else {
+      const uint16_t h = (uint16_t)(w[i / 2] >> (16 * (i % 2)));
+      return to_f32(*reinterpret_cast<const T*>(&h));
+    }
+  }
+  __device__ __forceinline__ void set2(int i, float x, float y) {  // elements i and i + 1, i even
+    if constexpr (sizeof(T) == 4) {
+      w[i] = __float_as_uint(x);
+      w[i + 1] = __float_as_uint(y);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const __half2 h = __floats2half2_rn(x, y);
+      w[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+      w[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void move(Raw<T, V>* dst, const Raw<T, V>* src) {  // one access each way
+  constexpr int B = Raw<T, V>::kBytes;
+  if constexpr (B >= 16) {
+#pragma unroll
+    for (int i = 0; i < B / 16; ++i) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
+  } else if constexpr (B == 8) {
+    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(src);
+  } else if constexpr (B == 4) {
+    *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
+  } else {
+    *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(src);
+  }
 }
 
 inline bool aligned_to(const void* p, uintptr_t n) {

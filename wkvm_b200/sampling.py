@@ -68,8 +68,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
         stride = V
     if u.dtype is not torch.float32 or not u.is_contiguous():
         u = u.to(torch.float32).contiguous()
-    tokens = torch.empty(B, dtype=torch.int64, device=logits.device)
-    logprobs = torch.empty(B, dtype=torch.float32, device=logits.device)
+    tokens, logprobs = torch.empty_like(u, dtype=torch.int64), torch.empty_like(u)
     p = _ops._ptr
     _ops._launch("wkvm_sample_tokens", idx, logits.data_ptr(), stride, u.data_ptr(), p(temp), p(k), p(tp), p(mp),
                  float(temp0), min(int(k0), V), float(tp0), float(mp0), tokens.data_ptr(), logprobs.data_ptr(), B, V,
