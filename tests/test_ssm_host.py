@@ -172,3 +172,14 @@ def test_c_entry_refusals(lib):
 
     assert sample(B=-1) == -1 and sample(V=0) == -1 and sample(dt=5) == -3 and sample(x=n) == -1
     assert sample(u=n) == -1 and sample(o=n) == -1 and sample(B=0) == 0
+
+
+def test_bank_layout():
+    from wkvm_b200.state import SSMStateBank, SSMStateLayout
+    lay = SSMStateLayout(2, 24, 8, 3, torch.float16)
+    bank = SSMStateBank(lay, num_slots=3, device="cpu")
+    assert bank.ssm.shape == (2, 4, 24, 8) and bank.conv.shape == (2, 4, 2, 24) and bank.conv.dtype == torch.float16
+    with pytest.raises(ValueError, match="multiples of 16 bytes"):
+        SSMStateLayout(2, 25, 16, 4)
+    with pytest.raises(_lib.WkvmError, match="SLOT_RANGE"):
+        bank.device_ids([4])

@@ -55,40 +55,60 @@ template <typename T, int N, int J>
 __global__ void __launch_bounds__(kRowThreads) scan_rows_kernel(ScanArgs p) {
   constexpr int LPC = N / 4;  // lanes of a channel
   constexpr int STEP = kRowThreads / LPC, CPB = STEP * J;
+  constexpr int CPT = (CPB + kRowThreads - 1) / kRowThreads;  // channels whose step a thread computes
   __shared__ float4 s_ch[CPB];  // delta, delta x, D x, gate
   __shared__ float s_y[CPB];
   const int n = blockIdx.x % p.seqs.nseq, c0 = blockIdx.x / p.seqs.nseq * CPB;
   const int tid = threadIdx.x, lane = tid % LPC, ch = tid / LPC;
+  const int live = p.D - c0 < CPB ? p.D - c0 : CPB;  // channels of this block
+  // everything that needs no slot id goes out ahead of the state
+  const T* xp = static_cast<const T*>(p.x.p) + n * p.x.bs + c0 + tid;
+  const T* dp = static_cast<const T*>(p.dt.p) + n * p.dt.bs + c0 + tid;
+  const T* zp = static_cast<const T*>(p.z.p) + n * p.z.bs + c0 + tid;
+  T xr[CPT], dr[CPT], zr[CPT];
+  auto load_token = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < CPT; ++i) {
+      if (tid + i * kRowThreads >= live) break;
+      xr[i] = xp[t * p.x.ts + i * kRowThreads];
+      dr[i] = dp[t * p.dt.ts + i * kRowThreads];
+      if (p.z.p) zr[i] = zp[t * p.z.ts + i * kRowThreads];
+    }
+  };
+  if (p.seqs.T > 0) load_token(0);
   int64_t row;
   if (!state_row(p.ids, p.num_slots, n, &row)) {
     if (tid == 0) report(p.status, WKVM_ERR_SLOT_RANGE);
     return;
   }
-  const int live = p.D - c0 < CPB ? p.D - c0 : CPB;  // channels of this block
   const int64_t hoff = (row * p.D + c0 + ch) * N + lane * 4;
-  const float* ap = p.A + (int64_t)(c0 + ch) * N + lane * 4;
-  float4 h[J];
+  float4 h[J], a[J];
 #pragma unroll
   for (int j = 0; j < J; ++j) {
     h[j] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (p.h_in && ch + j * STEP < live) h[j] = ld_stream_f4(p.h_in + hoff + j * STEP * N);
   }
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+    if (ch + j * STEP < live)
+      a[j] = *reinterpret_cast<const float4*>(p.A + (int64_t)(c0 + ch + j * STEP) * N + lane * 4);
   const int per_group = p.D / p.G;
-  const T* xp = static_cast<const T*>(p.x.p) + n * p.x.bs + c0;
-  const T* dp = static_cast<const T*>(p.dt.p) + n * p.dt.bs + c0;
-  const T* zp = static_cast<const T*>(p.z.p) + n * p.z.bs + c0;
   const T* bp = static_cast<const T*>(p.B.p) + n * p.B.bs + lane * 4;
   const T* cp = static_cast<const T*>(p.C.p) + n * p.C.bs + lane * 4;
   T* op = static_cast<T*>(p.o) + (int64_t)n * p.seqs.T * p.D + c0;
   const bool one_group = c0 / per_group == (c0 + live - 1) / per_group;
   for (int t = 0; t < p.seqs.T; ++t) {
-    for (int c = tid; c < live; c += kRowThreads) {
-      const float x = to_f32(xp[t * p.x.ts + c]);
-      float delta = to_f32(dp[t * p.dt.ts + c]) + (p.bias ? p.bias[c0 + c] : 0.f);
+#pragma unroll
+    for (int i = 0; i < CPT; ++i) {
+      const int c = tid + i * kRowThreads;
+      if (c >= live) break;
+      const float x = to_f32(xr[i]);
+      float delta = to_f32(dr[i]) + (p.bias ? p.bias[c0 + c] : 0.f);
       if (p.softplus) delta = softplus(delta);
-      const float gate = p.z.p ? silu<true>(to_f32(zp[t * p.z.ts + c])) : 1.f;
+      const float gate = p.z.p ? silu<true>(to_f32(zr[i])) : 1.f;
       s_ch[c] = make_float4(delta, delta * x, p.skip ? p.skip[c0 + c] * x : 0.f, gate);
     }
+    if (t + 1 < p.seqs.T) load_token(t + 1);
     __syncthreads();
     float bv[4], cv[4];
     int g = c0 / per_group;
@@ -110,11 +130,10 @@ __global__ void __launch_bounds__(kRowThreads) scan_rows_kernel(ScanArgs p) {
           read_bc();
         }
         const float2 s = *reinterpret_cast<const float2*>(&s_ch[c]);
-        const float4 a = *reinterpret_cast<const float4*>(ap + j * STEP * N);
-        h[j].x = fmaf(ex2(s.x * scaled(a.x)), h[j].x, s.y * bv[0]);
-        h[j].y = fmaf(ex2(s.x * scaled(a.y)), h[j].y, s.y * bv[1]);
-        h[j].z = fmaf(ex2(s.x * scaled(a.z)), h[j].z, s.y * bv[2]);
-        h[j].w = fmaf(ex2(s.x * scaled(a.w)), h[j].w, s.y * bv[3]);
+        h[j].x = fmaf(ex2(s.x * scaled(a[j].x)), h[j].x, s.y * bv[0]);
+        h[j].y = fmaf(ex2(s.x * scaled(a[j].y)), h[j].y, s.y * bv[1]);
+        h[j].z = fmaf(ex2(s.x * scaled(a[j].z)), h[j].z, s.y * bv[2]);
+        h[j].w = fmaf(ex2(s.x * scaled(a[j].w)), h[j].w, s.y * bv[3]);
         y = fmaf(h[j].x, cv[0], h[j].y * cv[1]) + fmaf(h[j].z, cv[2], h[j].w * cv[3]);
       }
 #pragma unroll
@@ -653,8 +672,10 @@ template <typename T, int N>
 int launch_scan_n(const ScanArgs& a, cudaStream_t st) {
   // a few tokens of every row: the state's traffic decides, so the row kernel
   if (!a.seqs.cu && a.seqs.T <= 8) {
-    // eight channels a thread once that still gives every SM its threads
-    if ((int64_t)a.seqs.nseq * a.D * N / 4 >= 148 * 1024 * 8) return launch_rows<T, N, 8>(a, st);
+    // Four channels a thread once that still gives every SM a thousand threads
+    // (512 rows of 4096 x 16: 72 us, 60 % of the measured HBM rate; two 92 us;
+    // eight 113 us, as A and the states then take 162 registers).
+    if ((int64_t)a.seqs.nseq * a.D * N / 16 >= 148 * 1024) return launch_rows<T, N, 4>(a, st);
     return launch_rows<T, N, 1>(a, st);
   }
   // Warps that four states (two channels) a thread give, of 592 schedulers.

@@ -25,6 +25,7 @@ from __future__ import annotations
 import torch
 
 from . import fla_compat, ops
+from .sampling import sample_tokens
 
 
 class GraphedDecode:
@@ -75,6 +76,18 @@ class GraphedDecode:
         next-token logits ``[len(slot_batch), vocab]``. The graph was captured
         with ``fla_compat`` installed as chosen at construction; it replays
         the same kernels whatever is installed now."""
+        return self._replay(slot_batch, last_tokens).float()
+
+    @torch.inference_mode()
+    def sample_step(self, slot_batch: list[dict[str, int]], last_tokens: list[int], u: torch.Tensor,
+                    temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> tuple[torch.Tensor, torch.Tensor]:
+        """:meth:`decode_step` and the choice of the next tokens, as
+        :meth:`wkvm_b200.runner.RWKV7Runner.sample_step`; the logits are read
+        in the model's dtype, which changes nothing."""
+        return sample_tokens(self._replay(slot_batch, last_tokens), u, temperature=temperature, top_k=top_k,
+                             top_p=top_p, min_p=min_p)
+
+    def _replay(self, slot_batch: list[dict[str, int]], last_tokens: list[int]) -> torch.Tensor:
         n = len(slot_batch)
         if n != len(last_tokens):
             raise ValueError("slot_batch and last_tokens length mismatch")
@@ -101,4 +114,4 @@ class GraphedDecode:
         self._staged = torch.cuda.Event()
         self._staged.record(torch.cuda.current_stream(dev))
         self.graph.replay()
-        return self.logits[:n, -1].float()
+        return self.logits[:n, -1]

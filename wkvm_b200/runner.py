@@ -21,6 +21,7 @@ from __future__ import annotations
 import torch
 
 from . import fla_compat
+from .sampling import sample_tokens
 
 
 class RWKV7Runner:
@@ -77,3 +78,13 @@ class RWKV7Runner:
                          logits_to_keep=1)
         self.bank.scatter_cache(slot_batch, cache)
         return out.logits[:, -1].float()
+
+    @torch.inference_mode()
+    def sample_step(self, slot_batch: list[dict[str, int]], last_tokens: list[int], u: torch.Tensor,
+                    temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> tuple[torch.Tensor, torch.Tensor]:
+        """:meth:`decode_step` and the choice of the next tokens from the
+        uniform numbers ``u`` [batch] (:func:`wkvm_b200.sample_tokens`, whose
+        settings are numbers or one value per row). Returns (tokens int64
+        [batch], log-probabilities fp32 [batch]) on the device."""
+        return sample_tokens(self.decode_step(slot_batch, last_tokens), u, temperature=temperature, top_k=top_k,
+                             top_p=top_p, min_p=min_p)

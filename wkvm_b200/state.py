@@ -18,7 +18,7 @@ from typing import Mapping, Sequence
 
 import torch
 
-from . import ops
+from . import ops, ssm
 
 WKV_DTYPE = torch.float32
 
@@ -207,6 +207,103 @@ class RWKV7StateBank:
     def state_bytes(self) -> int:
         return (self.wkv.numel() * self.wkv.element_size()
                 + self.shift.numel() * self.shift.element_size())
+
+
+@dataclass(frozen=True)
+class SSMStateLayout:
+    """Per-slot state shapes of selective state space layers: ``d_inner``
+    channels of ``d_state`` states, and the last ``d_conv - 1`` inputs of the
+    short convolution in the model's dtype."""
+
+    n_layer: int
+    d_inner: int
+    d_state: int = 16
+    d_conv: int = 4
+    dtype: torch.dtype = torch.bfloat16
+
+    def __post_init__(self) -> None:
+        row = (self.d_conv - 1) * self.d_inner * torch.empty((), dtype=self.dtype).element_size()
+        if row % 16 or self.d_inner * self.d_state % 4:
+            raise ValueError("a slot's rows must be multiples of 16 bytes (the slot copies move whole vectors): "
+                             f"{row} bytes of convolution inputs, {self.d_inner * self.d_state * 4} of states")
+
+    @property
+    def ssm_shape(self) -> tuple[int, int]:
+        return (self.d_inner, self.d_state)
+
+    @property
+    def conv_shape(self) -> tuple[int, int]:
+        return (self.d_conv - 1, self.d_inner)
+
+
+class SSMStateBank:
+    """Slot-indexed states of selective state space layers, with the slot
+    operations of :class:`RWKV7StateBank`:
+
+      ssm  [L, S+1, D, N] fp32          (slot 0 = reserved padding row)
+      conv [L, S+1, W-1, D] model dtype (the last W-1 inputs, oldest first)
+
+    ``conv`` / ``scan`` run one layer's short convolution and selective scan
+    for a batch of slots (``decode`` for new tokens, ``prefill`` for prompts),
+    states read and written in place."""
+
+    FAMILIES = (("ssm", 1), ("conv", 1))  # (tensor, slot axis)
+
+    def __init__(self, layout: SSMStateLayout, num_slots: int, device: torch.device | str = "cuda") -> None:
+        self.layout = layout
+        self.num_slots = num_slots
+        self.device = torch.device(device)
+        self.ssm = torch.zeros((layout.n_layer, num_slots + 1, *layout.ssm_shape), dtype=torch.float32,
+                               device=self.device)
+        self.conv = torch.zeros((layout.n_layer, num_slots + 1, *layout.conv_shape), dtype=layout.dtype,
+                                device=self.device)
+
+    def device_ids(self, slots: Sequence[int]) -> torch.Tensor:
+        """Validated int32 device ids for a batch (reuse across layers/steps)."""
+        return ops.slot_ids_tensor(slots, self.num_slots + 1, self.device)
+
+    # -- one layer --------------------------------------------------------
+
+    def conv_decode(self, layer: int, slot_ids, x, weight, bias=None, activation="silu") -> torch.Tensor:
+        return ssm.short_conv_decode_slots(x, weight, self.conv, layer, slot_ids, bias=bias, activation=activation)
+
+    def conv_prefill(self, layer: int, slot_ids, x, weight, bias=None, activation="silu",
+                     cu_seqlens=None) -> torch.Tensor:
+        return ssm.short_conv_prefill_slots(x, weight, self.conv, layer, slot_ids, bias=bias, activation=activation,
+                                            cu_seqlens=cu_seqlens)
+
+    def scan_decode(self, layer: int, slot_ids, x, dt, A, B, C, **more) -> torch.Tensor:
+        """``more``: D, z, dt_bias, dt_softplus of :func:`~wkvm_b200.ssm.selective_scan`."""
+        return ssm.selective_scan_decode_slots(x, dt, A, B, C, self.ssm, layer, slot_ids, **more)
+
+    def scan_prefill(self, layer: int, slot_ids, x, dt, A, B, C, cu_seqlens=None, **more) -> torch.Tensor:
+        return ssm.selective_scan_prefill_slots(x, dt, A, B, C, self.ssm, layer, slot_ids, cu_seqlens=cu_seqlens,
+                                                **more)
+
+    # -- slot lifecycle ---------------------------------------------------
+
+    def zero(self, slots: Sequence[int]) -> None:
+        for name, dim in self.FAMILIES:
+            ops.slot_zero(getattr(self, name), dim, slots)
+
+    def fork(self, parents: Sequence[int], children: Sequence[int]) -> None:
+        for name, dim in self.FAMILIES:
+            ops.slot_copy(getattr(self, name), dim, parents, children)
+
+    def snapshot(self, slots: Sequence[int]) -> dict[str, torch.Tensor]:
+        """Pinned host copies {"ssm": [n, L, D, N], "conv": [n, L, W-1, D]}. Synchronises."""
+        got = {name: ops.slot_snapshot(getattr(self, name), dim, slots) for name, dim in self.FAMILIES}
+        torch.cuda.current_stream(self.device).synchronize()
+        return got
+
+    def restore(self, slots: Sequence[int], tensors: Mapping[str, torch.Tensor]) -> None:
+        """Inverse of :meth:`snapshot`. Synchronises."""
+        for name, dim in self.FAMILIES:
+            ops.slot_restore(getattr(self, name), dim, slots, _pinned(tensors[name]))
+        torch.cuda.current_stream(self.device).synchronize()
+
+    def state_bytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.ssm, self.conv))
 
 
 def _pinned(t: torch.Tensor) -> torch.Tensor:
