@@ -682,16 +682,23 @@ int launch_scan_n(const ScanArgs& a, cudaStream_t st) {
   // Few: sequences are split in time over clusters (one of 8192 x 4096: 469 us
   // against 650 whole). A split pays twice for the exponentials, so it takes
   // four parts at least and room for them. Sequences of unequal length, or not
-  // enough rows for two waves: two states a thread, twice the warps (sixteen
-  // packed prompts of 32768 x 2048 in all: 630 us against 790). Else four (16
-  // equal ones of 2048: 500 us against 635).
-  constexpr int kFine = N == 128 ? 4 : 2, kWide = 2 * kFine;
+  // enough rows for two waves: fewer states a thread, so more warps (sixteen
+  // packed prompts of 32768 x 2048 in all: 630 us against 790). Else the wide
+  // form (16 equal ones of 2048: 500 us against 635). From 64 states on B and C
+  // outweigh a CTA's channels, so the fine form keeps four or eight states
+  // (three sequences of 666 x 1002, fp32: 110 us against 145 with two).
+  constexpr int kWide = N == 128 ? 8 : 4;
   const int64_t warps = (int64_t)a.seqs.nseq * a.D * N / (kWide * 2 * 32);
   const int64_t tokens = a.seqs.cu ? a.seqs.T / a.seqs.nseq : a.seqs.T;
   int parts = 1;
   while (parts < 16 && warps * parts * 2 <= 2048 && tokens >= parts * 8 * 16) parts *= 2;
   if (warps <= 256 && parts >= 4) return launch_tiles<T, N, 1, kWide, 64, 16, true>(a, parts, st);
-  if (a.seqs.cu || warps < 2048) return launch_tiles<T, N, 1, kFine, 64, 32, false>(a, 1, st);
+  if constexpr (N < 128) {
+    if (a.seqs.cu || warps < 2048) {
+      if constexpr (N == 64) return launch_tiles<T, N, 1, 4, 128, 32, false>(a, 1, st);
+      else return launch_tiles<T, N, 1, 2, 64, 32, false>(a, 1, st);
+    }
+  }
   return launch_tiles<T, N, 1, kWide, 64, 16, false>(a, 1, st);
 }
 
