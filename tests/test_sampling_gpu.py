@@ -58,7 +58,7 @@ def test_against_definition(cuda, setting, dtype, V):
     _check(x, u, **setting)
 
 
-@pytest.mark.parametrize("V", [1, 2, 3, 32, 33, 127, 1024, 1025, 4097, 16383, 16385, 40000, 131071, 200001])
+@pytest.mark.parametrize("V", [1, 2, 3, 32, 33, 127, 1024, 1025, 4097, 16383, 16385, 40000, 131071, 200001, 262144, 300008, 400001])
 def test_vocabulary_sizes(cuda, V):
     x, u = _logits(3, V, V, cuda, BF)
     for s in (dict(), dict(top_p=0.9), dict(top_k=20, top_p=0.8), dict(temperature=0)):
@@ -121,6 +121,39 @@ def test_masked_and_special_values(cuda):
     z = torch.zeros(2, V, device=cuda)
     z[:, 1::2] = -0.0                            # zeros of both signs are equal
     _check(z, u[:2], top_k=3)
+
+
+def test_odd_settings(cuda):
+    """Numbers outside [0, 1), settings that are NaN, negative or beyond the
+    vocabulary: each row still gets a token, as the settings' nearest meaning
+    has it."""
+    V = 2000
+    x, _ = _logits(6, V, 4, cuda, F32)
+    first, last = torch.full((6,), 0.0, device=cuda), torch.full((6,), 1 - 2.0 ** -24, device=cuda)
+    for s in (dict(), dict(top_k=9), dict(top_p=0.9), dict(min_p=0.01)):
+        a = wk.sample_tokens(x, first, **s)
+        for u in (-1.0, NAN, -INF):
+            b = wk.sample_tokens(x, torch.full((6,), u, device=cuda), **s)
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+        # at or past 1: the last kept id, which is never below the last number's
+        for u in (1.0, 2.0, INF):
+            b = wk.sample_tokens(x, torch.full((6,), u, device=cuda), **s)
+            assert bool((b[0] >= wk.sample_tokens(x, last, **s)[0]).all()) and bool((b[0] < V).all())
+            assert bool(b[1].isfinite().all())
+    u = torch.rand(6, device=cuda)
+    t = lambda v: torch.full((6,), v, device=cuda)  # noqa: E731
+    plain = wk.sample_tokens(x, u)
+    for s in (dict(top_p=t(NAN)), dict(min_p=t(NAN)), dict(min_p=t(-1.0)), dict(top_p=t(7.0)),
+              dict(top_k=torch.full((6,), -5, device=cuda)), dict(top_k=torch.full((6,), 10 ** 12, device=cuda))):
+        assert torch.equal(wk.sample_tokens(x, u, **s)[0], plain[0])
+    best = x.argmax(1)
+    for s in (dict(temperature=t(NAN)), dict(temperature=t(-1.0)), dict(top_p=t(-1.0)), dict(min_p=t(2.0)),
+              dict(top_k=1, top_p=0.5)):
+        assert torch.equal(wk.sample_tokens(x, u, **s)[0], best)
+    # a temperature without limit: every finite logit alike
+    x[:, 1000:] = -INF
+    tok, lp = wk.sample_tokens(x, u, temperature=t(INF))
+    assert torch.equal(tok, (u.double() * 1000).long()) and bool(((lp + math.log(1000)).abs() < 1e-6).all())
 
 
 def test_wide_ranges(cuda):

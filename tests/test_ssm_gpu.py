@@ -196,6 +196,76 @@ def test_scan_strided_views(cuda, T, rank):
     assert torch.equal(o3, o2)
 
 
+@pytest.mark.parametrize("dtype,D,N,G", [(BF, 64, 16, 1), (F32, 37, 8, 1), (FH, 40, 64, 2), (BF, 12, 128, 1), (F32, 24, 32, 3)])
+@pytest.mark.parametrize("lengths", [[900, 0, 3, 700, 1201], [2100], [1025, 1023]])
+def test_scan_long_rows_split_in_time(cuda, dtype, D, N, G, lengths):
+    """Few rows of many tokens: their parts run side by side; short sequences
+    among them leave parts empty."""
+    a = _scan_inputs(cuda, (1, sum(lengths)), D, N, G, dtype, seed=D)
+    cu, n = _cu(lengths, cuda), len(lengths)
+    h0 = torch.randn(n, D, N, device=cuda)
+    bank, ids = torch.zeros(1, n + 1, D, N, device=cuda), _ids(n, n)
+    bank[0, ids] = h0
+    o = wk.selective_scan_prefill_slots(*[a[k] for k in ("x", "dt", "A", "B", "C")], bank, 0, ids, D=a["D"], z=a["z"],
+                                        dt_bias=a["dt_bias"], cu_seqlens=cu)
+    ro, tol, rh, htol = _ref(a, h0, cu)
+    # a part's decay is the exponential of a sum of up to 2101 / 4 steps, each
+    # rounded once: 2^-24 of it a step at most, 2^-15 in all, on what came before
+    ssm_ref.check(o, ro, tol + 2.0 ** -15 * ro.abs().max() * (dtype == F32), "o")
+    ssm_ref.check(bank[0, ids], rh, htol + 2.0 ** -15 * h0.abs().max().double().cpu(), "state")
+    ops.check_device_status(cuda)
+
+
+def test_scan_pieces_and_steps_agree(cuda):
+    """A prompt at once, in pieces of every kind, and token by token."""
+    D, N, T = 40, 16, 600
+    a = _scan_inputs(cuda, (2, T), D, N, 2, F32, seed=9)
+    names = ("x", "dt", "B", "C", "z")
+    run = lambda fn, bank, lo, hi: fn(*[a[k][:, lo:hi] if k in names else a[k] for k in ("x", "dt", "A", "B", "C")],  # noqa: E731
+                                      bank, 0, [2, 1], D=a["D"], z=a["z"][:, lo:hi], dt_bias=a["dt_bias"])
+    ro, tol, rh, htol = _ref(a, torch.zeros(2, D, N))
+    cuts = [0, 1, 9, 17, 19, 300, T]
+    for bounds, fn in (([0, T], wk.selective_scan_prefill_slots), (cuts, wk.selective_scan_prefill_slots),
+                       (list(range(T + 1)), wk.selective_scan_decode_slots)):
+        bank = torch.zeros(1, 3, D, N, device=cuda)
+        o = torch.cat([run(fn, bank, lo, hi) for lo, hi in zip(bounds, bounds[1:])], 1)
+        ssm_ref.check(o, ro, tol, f"o in {len(bounds) - 1} pieces")
+        ssm_ref.check(bank[0, [2, 1]], rh, htol, "state")
+
+
+@pytest.mark.parametrize("dtype,B,T,D,N,G,skew", [(BF, 64, 41, 2048, 16, 1, 0), (FH, 64, 17, 2048, 16, 4, 3),
+                                                  (F32, 90, 33, 1001, 32, 1, 0), (BF, 33, 20, 2050, 64, 2, 0),
+                                                  (BF, 40, 35, 1030, 128, 1, 0), (FH, 130, 12, 2051, 8, 1, 1)])
+def test_scan_many_rows(cuda, dtype, B, T, D, N, G, skew):
+    """Enough rows for the wide launch shape, against the packed form of the
+    same sequences (another shape; the tests above hold that to 64 bits): the
+    same states to the bit, outputs within their sums' order."""
+    a = _scan_inputs(cuda, (B, T), D + skew, N, 1, dtype, seed=B)
+    for k in ("x", "dt", "z"):
+        a[k] = a[k][..., skew:]
+    for k in ("D", "dt_bias"):
+        a[k] = a[k][skew:].contiguous()
+    a["A"] = a["A"][skew:].contiguous()
+    a["B"], a["C"] = (t.expand(B, T, G, N).contiguous() * torch.arange(1, G + 1, device=cuda).view(1, 1, G, 1).to(dtype)
+                      for t in (a["B"], a["C"]))
+    if D % G:
+        a["B"], a["C"] = a["B"][:, :, :1], a["C"][:, :, :1]
+    h0 = torch.randn(B, D, N, device=cuda)
+    more = {k: a[k] for k in ("D", "dt_bias")}
+    o, ht = wk.selective_scan(a["x"], a["dt"], a["A"], a["B"], a["C"], z=a["z"], initial_state=h0,
+                              output_final_state=True, **more)
+    flat = lambda t: t.reshape(1, B * T, *t.shape[2:])  # noqa: E731
+    cu = torch.arange(0, B * T + 1, T, device=cuda)
+    o2, ht2 = wk.selective_scan(flat(a["x"]), flat(a["dt"]), a["A"], flat(a["B"]), flat(a["C"]), z=flat(a["z"]),
+                                initial_state=h0, output_final_state=True, cu_seqlens=cu, **more)
+    assert torch.equal(ht, ht2)
+    # fp32 sums of N terms in two orders: N 2^-24 of their magnitudes, which stay
+    # below 2^7 of the largest output here; then half a step of each rounding
+    u = torch.finfo(dtype).eps / 2
+    w = o2.view(B, T, D).double()
+    assert bool(((o.double() - w).abs() <= 2 * u * w.abs() + N * 2.0 ** -17 * w.abs().max() * 2.0 ** -7).all())
+
+
 def test_scan_mixed_dtypes(cuda):
     """fp32 B and C beside bf16 activations: computed in fp32, returned in x's dtype."""
     a = _scan_inputs(cuda, (2, 9), 24, 16, 1, BF)

@@ -85,6 +85,7 @@ def test_scan_refusals(anywhere):
 
     bad = [
         (dict(x=torch.zeros(3, 12)), "x must be"),
+        (dict(x=torch.zeros(2, 3, 12, dtype=torch.float64)), "unsupported dtype"),
         (dict(dt=torch.zeros(2, 3, 1)), "dt must have x's shape"),
         (dict(z=torch.zeros(2, 4, 12)), "z must have x's shape"),
         (dict(A=torch.zeros(16, 12)), "A must be"),

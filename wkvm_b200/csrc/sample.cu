@@ -61,8 +61,8 @@ struct SampleArgs {
 constexpr int kNT = 512, kWarps = kNT / 32;
 constexpr int kBins = 1024;
 constexpr int kCap = 1024;        // candidates one CTA sorts
-constexpr int kGroups = 6;        // sets of 32, 16, .. 1 threads
-constexpr int kMaxCtas = 8;       // CTAs of a row (portable cluster size)
+constexpr int kGroups = 10;       // 1, 2, 4, .. 512 sets of a CTA's threads
+constexpr int kMaxCtas = 16;      // CTAs of a row (16: a cluster size that a kernel has to ask for)
 constexpr int kSmemSlice = 16384; // logits of a slice kept in shared memory (two CTAs an SM)
 
 // Ascending unsigned order of floats; -0 counts as 0, -inf and NaN as 0u.
@@ -92,6 +92,9 @@ __device__ __forceinline__ double exp2_neg(double t, const double* table) {
   return __hiloint2double(__double2hiint(w) + ((k >> 6) << 20), __double2loint(w));
 }
 
+// The next smaller double of a positive one.
+__device__ __forceinline__ double below(double x) { return __longlong_as_double(__double_as_longlong(x) - 1); }
+
 struct Found {          // what a level of a selection found, the same in every CTA
   int bin;              // the bin with the boundary; -1: everything is kept
   uint32_t above, in;   // candidates in the bins above it, and in it
@@ -111,7 +114,7 @@ struct alignas(16) Shared {
   };
   double exp2_table[64];            // 2^(i / 64)
   u64 warp_sum[kWarps];
-  uint32_t warp_u32[1 + kGroups][kWarps];
+  uint32_t warp_u32[7][kWarps];
   uint32_t peer_max[kMaxCtas], peer_least[kGroups][kMaxCtas];
   uint32_t peer_lo[kMaxCtas], peer_hi[kMaxCtas], peer_cnt[kMaxCtas];
   u64 peer_mass[kMaxCtas], peer_total[kMaxCtas];
@@ -463,7 +466,7 @@ __device__ void finish_list(R& r, int n, int k, double tp, double mp, double u, 
   scan_weights(r, n);
   const u64 z = s->weight[n - 1];
   double goal = u * (double)z;
-  if (!(goal < (double)z)) goal = (double)(z - 1);
+  if (!(goal < (double)z)) goal = below((double)z);
   for (int i = r.tid; i < n; i += kNT) {
     const u64 before = i ? s->weight[i - 1] : 0;
     if (s->weight[i] > before && (double)s->weight[i] > goal && !((double)before > goal)) {
@@ -665,18 +668,19 @@ __global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
   if constexpr (SMEM)
     for (int i = r.n + r.tid; i < p.slice; i += kNT) vals[i] = -INFINITY;
 
-  const double u = p.u[b];
+  const double u = fmax((double)p.u[b], 0.0);  // NaN counts as 0
   float temp = p.temperature ? p.temperature[b] : p.temperature0;
   int k = p.top_k ? p.top_k[b] : p.top_k0;
-  const double tp = p.top_p ? p.top_p[b] : p.top_p0, mp = p.min_p ? p.min_p[b] : p.min_p0;
+  const double tp = p.top_p ? p.top_p[b] : p.top_p0;
+  const double mp = fmax((double)(p.min_p ? p.min_p[b] : p.min_p0), 0.0);
   if (!(temp > 0.f)) k = 1;
 
-  // Maximum of the row. And, for sets of 32, 16, .. 1 threads: the least
+  // Maximum of the row. And, for 1 to 512 sets of a CTA's threads: the least
   // maximum over the sets. As many logits as there are sets are at least that
   // large, which bounds the k-th largest from below.
   uint32_t set = key_of(most);
 #pragma unroll
-  for (int g = kGroups - 1; g >= 0; --g) {  // sets of 32 >> g threads
+  for (int g = 5; g >= 0; --g) {  // sets of 32 >> g threads
     const uint32_t least = __reduce_min_sync(0xffffffffu, set);
     if (r.lane == 0) s->warp_u32[1 + g][r.warp] = least;
     if (g) set = max(set, __shfl_xor_sync(0xffffffffu, set, 32 >> g));
@@ -687,13 +691,18 @@ __global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
     s->n_list = 0;
   }
   __syncthreads();
-  if (r.warp <= kGroups) {
-    const uint32_t v = r.lane < kWarps ? s->warp_u32[r.warp][r.lane] : r.warp ? 0xffffffffu : 0u;
-    const uint32_t x = r.warp ? __reduce_min_sync(0xffffffffu, v) : __reduce_max_sync(0xffffffffu, v);
-    if (r.lane < r.ctas) {
-      Shared* o = r.peer(r.lane);
-      (r.warp ? o->peer_least[r.warp - 1] : o->peer_max)[r.rank] = x;
+  if (r.warp >= 1 && r.warp <= 5) {  // sets of less than a warp
+    const uint32_t x = __reduce_min_sync(0xffffffffu, r.lane < kWarps ? s->warp_u32[1 + r.warp][r.lane] : 0xffffffffu);
+    if (r.lane < r.ctas) r.peer(r.lane)->peer_least[4 + r.warp][r.rank] = x;
+  } else if (r.warp == 0) {  // of 1, 2, .. 16 warps: lanes 16 to 31 repeat the first
+    uint32_t x = s->warp_u32[0][r.lane % kWarps];
+#pragma unroll
+    for (int g = 4; g >= 0; --g) {
+      const uint32_t least = __reduce_min_sync(0xffffffffu, x);
+      if (r.lane < r.ctas) r.peer(r.lane)->peer_least[g][r.rank] = least;
+      if (g) x = max(x, __shfl_xor_sync(0xffffffffu, x, 16 >> g));
     }
+    if (r.lane < r.ctas) r.peer(r.lane)->peer_max[r.rank] = x;
   }
   r.sync();
   uint32_t top = 0;
@@ -732,7 +741,7 @@ __global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
   }
   if (k > 0 && k < p.V) {
     int g = 0;  // the largest sets that are at least k
-    while (g < kGroups && (r.ctas * kWarps << g) < k) ++g;
+    while (g < kGroups && (r.ctas << g) < k) ++g;
     uint32_t least = 0;
     if (g < kGroups) {
       least = 0xffffffffu;
@@ -741,7 +750,7 @@ __global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
     const float lo = least ? value_of(least) : -FLT_MAX;  // 0: an empty set among them
     // About g ln g of the logits reach the least of g maxima, whatever their
     // distribution: few enough for the list without a histogram.
-    if (least && (r.ctas * kWarps << g) <= 128) {
+    if (least && (r.ctas << g) <= 128) {
       gather(r, [&](float l) { return l >= lo; });
       const uint32_t found = r.peer(0)->n_list;
       r.sync();  // read before the first CTA goes on
@@ -798,7 +807,7 @@ __global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
   }
   for (int i = 0; i < r.warp; ++i) before += s->warp_sum[i];
   double goal = u * (double)z;
-  if (!(goal < (double)z)) goal = (double)(z - 1);
+  if (!(goal < (double)z)) goal = below((double)z);
   // the one block in which the running mass passes the goal is split again
   // over the warps of its CTA
   auto holds = [&](u64 from, u64 mass) { return mass && !((double)from > goal) && (double)(from + mass) > goal; };
@@ -847,15 +856,15 @@ __global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
 template <typename T, bool SMEM>
 int launch_on(const SampleArgs& a, int B, cudaStream_t st) {
   const int bytes = (int)sizeof(Shared) + (SMEM ? a.slice * 4 : 0);
-  if (SMEM) {
-    static std::atomic<uint64_t> done{0};  // a bit per device: the shared-memory limit is raised
-    int dev = 0;
-    WKVM_CUDA_TRY(cudaGetDevice(&dev));
-    if (dev >= 64 || !(done.load(std::memory_order_acquire) >> dev & 1)) {
+  static std::atomic<uint64_t> done{0};  // a bit per device: shared memory and large clusters are allowed
+  int dev = 0;
+  WKVM_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev >= 64 || !(done.load(std::memory_order_acquire) >> dev & 1)) {
+    if (SMEM)
       WKVM_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T, SMEM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)sizeof(Shared) + kSmemSlice * 4));
-      if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
-    }
+    WKVM_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T, SMEM>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((int64_t)B * a.ctas));
@@ -894,11 +903,11 @@ extern "C" int wkvm_sample_tokens(const void* logits, int64_t row_stride, const 
   if (!logits || !u || !tokens || !logprobs) return WKVM_ERR_INVALID_ARG;
   // Slices of 16,384 fit shared memory and spread the rows that need several
   // passes (256 mixed rows of 65,536: 98 us over four CTAs each, 158 whole, 117
-  // over eight). Few rows take more CTAs (one: 34 us over eight, 45 over four).
+  // over eight). Few rows take more CTAs (one: 34 us over eight, 45 over four),
+  // sixteen only where all are resident at once.
   int ctas = 1;
-  while (ctas < wkvm::kMaxCtas &&
-         (V > ctas * wkvm::kSmemSlice || ((int64_t)B * ctas <= 256 && V >= ctas * 2048)))
-    ctas *= 2;
+  while (ctas < 8 && (V > ctas * wkvm::kSmemSlice || ((int64_t)B * ctas <= 256 && V >= ctas * 2048))) ctas *= 2;
+  if (ctas == 8 && (B <= 8 || V > 8 * wkvm::kSmemSlice) && V >= 16384) ctas = 16;
   if ((int64_t)B * ctas > INT32_MAX) return WKVM_ERR_SHAPE;
   const int64_t es = dtype == WKVM_DTYPE_F32 ? 4 : 2;
   const int slice = ((V + ctas - 1) / ctas + wkvm::kNT - 1) / wkvm::kNT * wkvm::kNT;

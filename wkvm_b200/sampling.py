@@ -23,6 +23,8 @@ def _setting(name: str, value, rows: int, dtype: torch.dtype, logits: torch.Tens
         raise ValueError(f"{name} must be a number or [{rows}], not {tuple(value.shape)}")
     if value.dtype is dtype and value.get_device() == logits.get_device() and value.is_contiguous():
         return value, 0
+    if dtype is torch.int32 and value.dtype is not torch.int32:
+        value = value.clamp(0, (1 << 31) - 1)
     return value.to(device=logits.device, dtype=dtype).contiguous(), 0
 
 

@@ -246,7 +246,9 @@ class _Scan:
             if t is not None and (t.dim() != 1 or t.shape[0] != d):
                 raise ValueError(f"{name} must be [{d}], not {tuple(t.shape)}")
         self.dtype = dtype = x.dtype  # the output's
-        if (dtype not in _ops._DTYPES or dt.dtype is not dtype or B.dtype is not dtype or C.dtype is not dtype
+        if dtype not in _ops._DTYPES:
+            raise ValueError(f"unsupported dtype {dtype}")
+        if (dt.dtype is not dtype or B.dtype is not dtype or C.dtype is not dtype
                 or (z is not None and z.dtype is not dtype)):
             # mixed dtypes are widened to fp32 (lossless), as the other ops do
             x, dt, B, C, z = (None if t is None else t.float() for t in (x, dt, B, C, z))
