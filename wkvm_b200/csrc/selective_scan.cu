@@ -52,7 +52,7 @@ constexpr int kRowThreads = 128;
 __device__ __forceinline__ float scaled(float a) { return fmaxf(a * kLog2e, -FLT_MAX); }
 
 template <typename T, int N, int J>
-__global__ void __launch_bounds__(kRowThreads) scan_rows_kernel(ScanArgs p) {
+__global__ void __launch_bounds__(kRowThreads, 8) scan_rows_kernel(ScanArgs p) {
   constexpr int LPC = N / 4;  // lanes of a channel
   constexpr int STEP = kRowThreads / LPC, CPB = STEP * J;
   constexpr int CPT = (CPB + kRowThreads - 1) / kRowThreads;  // channels whose step a thread computes
@@ -673,7 +673,7 @@ int launch_scan_n(const ScanArgs& a, cudaStream_t st) {
   // a few tokens of every row: the state's traffic decides, so the row kernel
   if (!a.seqs.cu && a.seqs.T <= 8) {
     // Four channels a thread once that still gives every SM a thousand threads
-    // (512 rows of 4096 x 16: 72 us, 60 % of the measured HBM rate; two 92 us;
+    // (512 rows of 4096 x 16: 70 us, 62 % of the measured HBM rate; two 92 us;
     // eight 113 us, as A and the states then take 162 registers).
     if ((int64_t)a.seqs.nseq * a.D * N / 16 >= 148 * 1024) return launch_rows<T, N, 4>(a, st);
     return launch_rows<T, N, 1>(a, st);
