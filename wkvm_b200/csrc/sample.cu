@@ -27,7 +27,11 @@
 // then finish on a sorted list of at most kCap candidates in one CTA. Only a
 // larger set is narrowed by further histograms and drawn from by a pass over
 // the whole row. HBM is read once: later passes find the slice in shared
-// memory, or, in vocabularies too long for eight CTAs', in L2.
+// memory, or, in vocabularies too long for sixteen CTAs', in L2. At 256 rows of
+// 65,536 fp32 logits (10 us of HBM): 33 us greedy, 47 top-k 50, 70 without a
+// filter, 160 to 190 top-p 0.9 (thousands of tokens kept), which evaluates the
+// weights twice; the issue of some ninety instructions a logit bounds it, then
+// the latency of one row's phases (one row: 8, 16, 10 and 31 us).
 #include <cooperative_groups.h>
 #include <float.h>
 

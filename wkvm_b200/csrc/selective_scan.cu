@@ -153,8 +153,13 @@ __global__ void __launch_bounds__(kRowThreads, 8) scan_rows_kernel(ScanArgs p) {
 }
 
 // ---------------------------------------------------------------------------
-// Tile kernel, for prompts. T D N exponentials (16 a clock and SM) bound it:
-// 16 states give 4.65e12 / s against 8 bytes of activations per 16 of them.
+// Tile kernel, for prompts. Its floor is T D N exponentials at 16 a clock and
+// SM (4.65e12 / s; 231 us for 32768 x 2048 x 16) rather than the 8 bytes of
+// activations per N of them (83 us). What bounds it is the issue of the other
+// instructions, some nine an exponential: at sixteen packed prompts of that
+// size it takes 594 us, the exponentials' pipe half busy, 0.6 instructions a
+// clock and scheduler from three warps (two channels to a register pair took
+// it from 880 us, straight-line tile phases and byte permutes to 594).
 //
 // One CTA walks one sequence for CB channels, TT tokens at a time. A thread
 // keeps NS states of CH channels; the L = N / NS threads of a channel leave
