@@ -17,7 +17,7 @@ forward only: inputs that ask for gradients are refused.
 
 from __future__ import annotations
 
-import ctypes
+import struct
 
 import torch
 
@@ -27,7 +27,7 @@ from . import ops as _ops
 _STATES = (8, 16, 32, 64, 128)
 _WIDTHS = (2, 3, 4)
 _ACTIVATIONS = {None: 0, "silu": 1, "swish": 1}
-_Strides = ctypes.c_int64 * 10
+_strides = struct.Struct("10q").pack  # the C call's array of ten int64
 
 
 def _check(ts) -> int:
@@ -263,7 +263,7 @@ class _Scan:
         self.x = x
         # kept until the launch: some are copies made here
         self.inputs = (x, dt, _f32(A), B, C, _f32(D), z, _f32(dt_bias))
-        self.strides = _Strides(xs[0], xs[1], ds[0], ds[1], zs[0], zs[1], bs[0], bs[1], cs[0], cs[1])
+        self.strides = _strides(xs[0], xs[1], ds[0], ds[1], zs[0], zs[1], bs[0], bs[1], cs[0], cs[1])
 
     def output(self):
         return _new_like(self.x)
