@@ -65,6 +65,7 @@ struct SampleArgs {
 constexpr int kNT = 512, kWarps = kNT / 32;
 constexpr int kBins = 1024;
 constexpr int kCap = 1024;        // candidates one CTA sorts
+constexpr int kRankSort = 384;    // of which so many by counting
 constexpr int kGroups = 10;       // 1, 2, 4, .. 512 sets of a CTA's threads
 constexpr int kMaxCtas = 16;      // CTAs of a row (16: a cluster size that a kernel has to ask for)
 constexpr int kSmemSlice = 16384; // logits of a slice kept in shared memory (two CTAs an SM)
@@ -385,16 +386,34 @@ __device__ void gather(R& r, F take) {
 }
 
 // Sorts the first n entries of the list ascending (one CTA, n <= kCap).
-template <typename R>
-__device__ void sort_list(R& r, int n) {
-  Shared* s = r.s;
+__device__ __forceinline__ void sort_list(Shared* s, int tid, int n) {
+  if (n <= kRankSort) {
+    // few: every entry counts those ahead of it (they differ, by their ids);
+    // n reads without a barrier beat some forty steps that each wait
+    if (tid == 0) s->list[n] = ~0ull;  // an even number to read
+    __syncthreads();
+    if (tid < n) {
+      const u64 mine = s->list[tid];
+      int rank = 0;
+#pragma unroll 4
+      for (int i = 0; i < n; i += 2) {
+        const ulonglong2 e = *reinterpret_cast<const ulonglong2*>(&s->list[i]);
+        rank += (e.x < mine) + (e.y < mine);
+      }
+      s->weight[rank] = mine;
+    }
+    __syncthreads();
+    if (tid < n) s->list[tid] = s->weight[tid];
+    __syncthreads();
+    return;
+  }
   int size = 2;
   while (size < n) size *= 2;
-  for (int i = n + r.tid; i < size; i += kNT) s->list[i] = ~0ull;
+  for (int i = n + tid; i < size; i += kNT) s->list[i] = ~0ull;
   __syncthreads();
   // thread t compares the pair at a = 2t with bit j cleared: with j <= 32 a
   // warp's pairs are its own 64 entries, and only wider steps meet the others
-  const int t = r.tid;
+  const int t = tid;
   for (int k = 2; k <= size; k *= 2)
     for (int j = k / 2; j > 0; j /= 2) {
       if (t < size / 2) {
@@ -411,21 +430,19 @@ __device__ void sort_list(R& r, int n) {
 }
 
 // Inclusive sums of weight[0, n) in place (one CTA, two neighbours a thread).
-template <typename R>
-__device__ void scan_weights(R& r, int n) {
-  Shared* s = r.s;
-  const int i = 2 * r.tid;
+__device__ __forceinline__ void scan_weights(Shared* s, int tid, int n) {
+  const int i = 2 * tid;
   const u64 a = i < n ? s->weight[i] : 0, b = i + 1 < n ? s->weight[i + 1] : 0;
   u64 x = a + b;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
     const u64 up = __shfl_up_sync(0xffffffffu, x, off);
-    if (r.lane >= off) x += up;
+    if ((tid & 31) >= off) x += up;
   }
   __syncthreads();
-  if (r.lane == 31) s->warp_sum[r.warp] = x;
+  if ((tid & 31) == 31) s->warp_sum[(tid >> 5)] = x;
   __syncthreads();
-  for (int w = 0; w < r.warp; ++w) x += s->warp_sum[w];
+  for (int w = 0; w < (tid >> 5); ++w) x += s->warp_sum[w];
   if (i < n) s->weight[i] = x - b;
   if (i + 1 < n) s->weight[i + 1] = x;
   __syncthreads();
@@ -439,13 +456,13 @@ template <typename R>
 __device__ void finish_list(R& r, int n, int k, double tp, double mp, double u, u64 total,
                             int64_t* token, float* logprob) {
   Shared* s = r.s;
-  sort_list(r, n);
+  sort_list(s, r.tid, n);
   if (k < n) n = k;
   auto weigh = [&](int i) { return r.weight(value_of(list_key(s->list[i]))); };
   if (tp < 1.0) {
     for (int i = r.tid; i < n; i += kNT) s->weight[i] = r.units(weigh(i));
     __syncthreads();
-    scan_weights(r, n);
+    scan_weights(s, r.tid, n);
     const double goal = tp * (double)(total ? total : s->weight[n - 1]);
     // entry i stays while the mass before it is short of the goal
     uint32_t stay = 0;
@@ -463,11 +480,11 @@ __device__ void finish_list(R& r, int n, int k, double tp, double mp, double u, 
     s->list[i] = (e << 32) | (e >> 32);
   }
   __syncthreads();
-  sort_list(r, n);
+  sort_list(s, r.tid, n);
   auto by_id = [&](int i) { return r.weight(value_of(~(uint32_t)s->list[i])); };
   for (int i = r.tid; i < n; i += kNT) s->weight[i] = r.units(by_id(i));
   __syncthreads();
-  scan_weights(r, n);
+  scan_weights(s, r.tid, n);
   const u64 z = s->weight[n - 1];
   double goal = u * (double)z;
   if (!(goal < (double)z)) goal = below((double)z);
@@ -552,10 +569,10 @@ __device__ bool select(R& r, float lo, double goal, int k, double tp, double mp,
       gather(r, [&](float l) { return b.holds(l) && b(l) == f.bin; });
       if (r.rank == 0) {
         const int n = (int)f.in;
-        sort_list(r, n);
+        sort_list(s, r.tid, n);
         for (int i = r.tid; i < n; i += kNT) s->weight[i] = MASS ? r.units(r.weight(value_of(list_key(s->list[i])))) : 1;
         __syncthreads();
-        scan_weights(r, n);
+        scan_weights(s, r.tid, n);
         const u64 base = MASS ? f.mass_above : f.above;
         for (int i = r.tid; i < n; i += kNT) {
           const double before = (double)(base + (i ? s->weight[i - 1] : 0));

@@ -89,35 +89,30 @@ __global__ void __launch_bounds__(kThreads) short_conv_kernel(ConvArgs p) {
   const T* wp = static_cast<const T*>(p.w);
   const T* xp = static_cast<const T*>(p.x.p);
   T* op = static_cast<T*>(p.o);
-  Pair<V> w[W][P], bias[P], win[W][P];  // win: the window, oldest first
+  Pair<V> w[W][P], win[W][P];  // win: the window, oldest first
+  Raw<T, V> wr[W], br;         // weights and bias as they lie in memory
 
-  auto load_weights = [&](int c) {
-    const T* src = wp + (int64_t)c * W;  // channel-major: V * W contiguous weights
-    Raw<T, V> r[W];
-#pragma unroll
-    for (int j = 0; j < W; ++j) r[j] = load_raw<T, V>(src + j * V);
-    auto at = [&](int i, int j) { return r[(i * W + j) / V].f32((i * W + j) % V); };  // channel i, tap j
-#pragma unroll
-    for (int j = 0; j < W; ++j)
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        if constexpr (V == 1) w[j][i] = at(0, j);
-        else w[j][i] = pack2(at(2 * i, j), at(2 * i + 1, j));
-      }
-#pragma unroll
-    for (int i = 0; i < P; ++i) bias[i] = 0;
-    if (p.bias) widen<T, V>(load_raw<T, V>(static_cast<const T*>(p.bias) + c), bias);
+  // pair (or channel) i of the weights of tap j: V * W weights, channel-major
+  auto weight = [&](int j, int i) -> Pair<V> {
+    auto at = [&](int c) { return wr[(c * W + j) / V].f32((c * W + j) % V); };
+    if constexpr (V == 1) return at(0);
+    else return pack2(at(2 * i), at(2 * i + 1));
   };
-  auto emit = [&](int64_t token, int c) {
-    Pair<V> y[P];
+  auto load_weights = [&](int c) {
+    const T* src = wp + (int64_t)c * W;
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-      y[i] = bias[i];
+    for (int j = 0; j < W; ++j) wr[j] = load_raw<T, V>(src + j * V);
 #pragma unroll
-      for (int j = 0; j < W; ++j) y[i] = fma_(w[j][i], win[j][i], y[i]);
-      if (SILU) y[i] = silu_of<sizeof(T) == 4>(y[i]);
+    for (int i = 0; i < Raw<T, V>::kWords; ++i) br.w[i] = 0;
+    if (p.bias) br = load_raw<T, V>(static_cast<const T*>(p.bias) + c);
+    if constexpr (TILES) {  // used again and again: widened once
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+#pragma unroll
+        for (int i = 0; i < P; ++i) w[j][i] = weight(j, i);
     }
-    T* dst = op + token * p.D + c;
+  };
+  auto put = [&](T* dst, const Pair<V> (&y)[P]) {
     if constexpr (V == 1) {
       *dst = from_f32<T>(y[0]);
     } else {
@@ -129,6 +124,17 @@ __global__ void __launch_bounds__(kThreads) short_conv_kernel(ConvArgs p) {
       }
       move<T, V>(reinterpret_cast<Raw<T, V>*>(dst), &out);
     }
+  };
+  auto emit = [&](int64_t token, int c) {
+    Pair<V> y[P];
+    widen<T, V>(br, y);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+#pragma unroll
+      for (int j = 0; j < W; ++j) y[i] = fma_(TILES ? w[j][i] : weight(j, i), win[j][i], y[i]);
+      if (SILU) y[i] = silu_of<sizeof(T) == 4>(y[i]);
+    }
+    put(op + token * p.D + c, y);
   };
   auto shift = [&](const Raw<T, V>& in) {
 #pragma unroll
@@ -170,23 +176,12 @@ __global__ void __launch_bounds__(kThreads) short_conv_kernel(ConvArgs p) {
       emit(sp.bos + t, c);
     }
     if (p.s_out) {
-      // the last W - 1 inputs: the sequence's own, ahead of them what it
-      // leaves of the row (read at j + len, so ahead of what is written)
+      // the last W - 1 inputs: those in the window, unless the sequence goes on
+      // in tile blocks
 #pragma unroll
       for (int j = 0; j + 1 < W; ++j) {
-        const int64_t t = sp.len - (W - 1) + j;
-        T* dst = static_cast<T*>(p.s_out) + srow + (int64_t)j * p.D;
-        Raw<T, V> in;
-#pragma unroll
-        for (int i = 0; i < Raw<T, V>::kWords; ++i) in.w[i] = 0;
-        if (t >= 0)
-          in = load_raw<T, V>(xs + t * p.x.ts);
-        else if (p.s_in)
-          in = load_raw<T, V>(static_cast<const T*>(p.s_in) + srow + (j + sp.len) * p.D);
-        if constexpr (Raw<T, V>::kBytes == 2)
-          *reinterpret_cast<uint16_t*>(dst) = (uint16_t)in.w[0];
-        else
-          move<T, V>(reinterpret_cast<Raw<T, V>*>(dst), &in);
+        if (head < sp.len) widen<T, V>(load_raw<T, V>(xs + (sp.len - (W - 1) + j) * p.x.ts), win[j + 1]);
+        put(static_cast<T*>(p.s_out) + srow + (int64_t)j * p.D, win[j + 1]);
       }
     }
     return;
