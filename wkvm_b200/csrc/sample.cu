@@ -28,14 +28,12 @@
 // larger set is narrowed by further histograms and drawn from by a pass over
 // the whole row. HBM is read once: later passes find the slice in shared
 // memory, or, in vocabularies too long for sixteen CTAs', in L2. At 256 rows of
-// 65,536 fp32 logits (10 us of HBM): 33 us greedy, 47 top-k 50, 70 without a
-// filter, 160 to 190 top-p 0.9 (thousands of tokens kept), which evaluates the
-// weights twice; the issue of some ninety instructions a logit bounds it, then
-// the latency of one row's phases (one row: 8, 16, 10 and 31 us).
+// 65,536 fp32 logits (10 us of HBM): 33 us greedy, 60 top-k 50, 70 without a
+// filter, 182 top-p 0.9 (thousands of tokens kept), which evaluates the weights
+// twice; the issue of some ninety instructions a logit bounds it, then the
+// latency of one row's phases (one row: 8, 14, 12 and 31 us).
 #include <cooperative_groups.h>
 #include <float.h>
-
-#include <atomic>
 
 #include "common.cuh"
 
@@ -877,16 +875,10 @@ __global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
 template <typename T, bool SMEM>
 int launch_on(const SampleArgs& a, int B, cudaStream_t st) {
   const int bytes = (int)sizeof(Shared) + (SMEM ? a.slice * 4 : 0);
-  static std::atomic<uint64_t> done{0};  // a bit per device: shared memory and large clusters are allowed
-  int dev = 0;
-  WKVM_CUDA_TRY(cudaGetDevice(&dev));
-  if (dev >= 64 || !(done.load(std::memory_order_acquire) >> dev & 1)) {
-    if (SMEM)
-      WKVM_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T, SMEM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)sizeof(Shared) + kSmemSlice * 4));
+  if (SMEM)
+    WKVM_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T, SMEM>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (a.ctas > 8)
     WKVM_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T, SMEM>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
-  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((int64_t)B * a.ctas));
   cfg.blockDim = dim3(kNT);

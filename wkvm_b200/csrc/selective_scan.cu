@@ -11,7 +11,6 @@
 #include <cooperative_groups.h>
 #include <float.h>
 
-#include <atomic>
 #include <type_traits>
 
 #include "ssm_common.cuh"
@@ -626,21 +625,6 @@ int launch_rows(const ScanArgs& a, cudaStream_t st) {
   return cudaGetLastError() == cudaSuccess ? WKVM_OK : WKVM_ERR_CUDA;
 }
 
-// Allows a kernel its shared memory (and clusters of 16) on the current
-// device, once each.
-template <auto Kernel>
-int allow(int bytes, bool big_cluster) {
-  static std::atomic<uint64_t> done{0};  // a bit per device
-  int dev = 0;
-  WKVM_CUDA_TRY(cudaGetDevice(&dev));
-  if (dev < 64 && (done.load(std::memory_order_acquire) >> dev & 1)) return WKVM_OK;
-  WKVM_CUDA_TRY(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  if (big_cluster)
-    WKVM_CUDA_TRY(cudaFuncSetAttribute(Kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-  if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
-  return WKVM_OK;
-}
-
 template <typename T, int N, int NP, int NS, int NT, int TT, bool CLUSTER>
 int launch_tiles(const ScanArgs& s, int parts, cudaStream_t st) {
   using K = Tile<T, N, NP, NS, NT, TT>;
@@ -658,7 +642,9 @@ int launch_tiles(const ScanArgs& s, int parts, cudaStream_t st) {
   if (jobs * parts > INT32_MAX) return WKVM_ERR_SHAPE;
   constexpr auto kern = scan_tiles_kernel<T, N, NP, NS, NT, TT, CLUSTER>;
   constexpr int bytes = K::bytes(CLUSTER);
-  if (int rc = allow<kern>(bytes, CLUSTER)) return rc;
+  WKVM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (CLUSTER)  // of 16
+    WKVM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(jobs * parts));
   cfg.blockDim = dim3(NT);

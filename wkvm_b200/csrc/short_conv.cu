@@ -8,8 +8,8 @@
 // convolution of selective state space layers and of gated-delta-rule layers.
 //
 // Streaming: every input is read once, every output written once, 2 W FLOPs
-// each, so HBM bounds it: sixteen packed prompts of 32768 x 4096 bf16 take 115
-// us, 4.7 TB/s or 71 % of the measured copy rate (218 us with one input in
+// each, so HBM bounds it: sixteen packed prompts of 32768 x 4096 bf16 take 118
+// us, 4.6 TB/s or 70 % of the measured copy rate (218 us with one input in
 // flight a thread and scalar arithmetic). One thread owns a few neighbouring channels and keeps
 // their weights and window in registers, two channels to a pair.
 //
