@@ -129,7 +129,7 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
 // V elements as they lie in memory, held as words: elements of 16 bits kept
 // apart would be taken apart, and so waited for, right after the load.
 template <typename T, int V>
-struct Raw {
+struct alignas(sizeof(T) * V >= 16 ? 16 : sizeof(T) * V <= 4 ? 4 : 8) Raw {
   static constexpr int kBytes = sizeof(T) * V, kWords = (kBytes + 3) / 4;
   uint32_t w[kWords];
   __device__ __forceinline__ float f32(int i) const {
