@@ -232,6 +232,15 @@ struct Row {
     for (int i = 0; i < kWarps; ++i) t += s->warp_sum[i];
     return t;
   }
+  // Another CTA's shared memory may be touched only once that CTA is known to
+  // run: behind wait_started(), or any sync(). Every thread arrives at the
+  // kernel's entry, so that loading the slice hides the wait.
+  __device__ void arrive_started() const {
+    if (ctas > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+  }
+  __device__ void wait_started() const {
+    if (ctas > 1) asm volatile("barrier.cluster.wait;" ::: "memory");
+  }
   __device__ Shared* peer(int r) const { return ctas == 1 ? s : cg::this_cluster().map_shared_rank(s, r); }
   __device__ void sync() const {  // the row's CTAs
     if (ctas == 1) __syncthreads(); else cg::this_cluster().sync();
@@ -644,6 +653,7 @@ __global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
   float* vals = reinterpret_cast<float*>(smem + sizeof(Shared));
   r.vals = vals;
   r.ctas = p.ctas;
+  r.arrive_started();
   r.rank = (int)(blockIdx.x % p.ctas);
   r.tid = threadIdx.x;
   r.lane = r.tid & 31;
@@ -710,6 +720,7 @@ __global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
     s->n_list = 0;
   }
   __syncthreads();
+  r.wait_started();
   if (r.warp >= 1 && r.warp <= 5) {  // sets of less than a warp
     const uint32_t x = __reduce_min_sync(0xffffffffu, r.lane < kWarps ? s->warp_u32[1 + r.warp][r.lane] : 0xffffffffu);
     if (r.lane < r.ctas) r.peer(r.lane)->peer_least[4 + r.warp][r.rank] = x;
