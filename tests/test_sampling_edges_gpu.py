@@ -1,7 +1,9 @@
 """Token sampling at the edges of what its documentation allows: rows whose
 CTAs start apart, two host threads, settings and numbers at their limits."""
 
+import ctypes
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -9,6 +11,7 @@ import torch
 
 import ssm_ref
 import wkvm_b200 as wk
+from wkvm_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +59,33 @@ def test_rows_whose_ctas_start_apart(cuda, B, V):
         tok, lp = wk.sample_tokens(x, u, **s)
         assert tok.tolist() == want.tolist() and _near(lp, wlp, V), i
     torch.cuda.synchronize()
+
+
+def test_threads_with_vocabularies_of_their_own(cuda):
+    """Host threads sample from vocabularies whose kernels need different
+    amounts of shared memory: no call makes another thread's fail. The C entry
+    is called without the interpreter's lock, as ctypes does."""
+    entry, f, p = _lib.load().wkvm_sample_tokens, ctypes.c_float, ctypes.c_void_p
+    sizes, wrong = (131072, 131072, 700, 700), []
+    start = threading.Barrier(len(sizes))
+
+    def serve(V):
+        with torch.cuda.device(cuda), torch.cuda.stream(torch.cuda.Stream(cuda)):
+            stream = torch.cuda.current_stream(cuda)
+            x, u = _logits(1, V, V, cuda, BF)
+            tok, lp = torch.empty(1, dtype=torch.int64, device=cuda), torch.empty(1, device=cuda)
+            args = (p(x.data_ptr()), V, p(u.data_ptr()), None, None, None, None, f(1), 0, f(0.9), f(0),
+                    p(tok.data_ptr()), p(lp.data_ptr()), 1, V, 1, None, p(stream.cuda_stream))
+            start.wait()
+            rc = [entry(*args) for _ in range(2000)]
+            stream.synchronize()
+            want, _ = _want(x, u, top_p=0.9)
+            if any(rc) or tok.tolist() != want.tolist():
+                wrong.append((V, sum(c != 0 for c in rc), tok.tolist(), want.tolist()))
+
+    threads = [threading.Thread(target=serve, args=(V,)) for V in sizes]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong

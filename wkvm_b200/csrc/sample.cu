@@ -886,8 +886,12 @@ __global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
 template <typename T, bool SMEM>
 int launch_on(const SampleArgs& a, int B, cudaStream_t st) {
   const int bytes = (int)sizeof(Shared) + (SMEM ? a.slice * 4 : 0);
+  // The limit belongs to the function and every host thread shares it, so it is
+  // the same constant whatever the call: a smaller one would refuse another
+  // thread's launch.
+  constexpr int most = (int)sizeof(Shared) + kSmemSlice * 4;
   if (SMEM)
-    WKVM_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T, SMEM>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    WKVM_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T, SMEM>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
   if (a.ctas > 8)
     WKVM_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T, SMEM>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg = {};
