@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(NT) scan_tiles_kernel(TileArgs q) {
     fz = zp ? zp + (int64_t)t0 * p.z.ts : nullptr;
     fb = bp + (int64_t)t0 * p.B.ts + tid * VB % N;
     fc = cp + (int64_t)t0 * p.C.ts + tid * VB % N;
-    out = op + (int64_t)(t0 + te) * p.D;
+    out = op + ((int64_t)t0 + te) * p.D;
     left = len - t0;
   };
   auto fetch = [&](int stage, bool emit) {
@@ -415,11 +415,13 @@ __global__ void __launch_bounds__(NT) scan_tiles_kernel(TileArgs q) {
   const float* src0 = sY + te * K::YROW + padded(ce * L);
   float* y0 = sY + padded(2 * tid);
   auto run = [&](int t0, int t1, bool emit) {
-    if (t0 >= t1) return;
+    // counted down: a tile's end may lie past the last int32
+    int todo = t1 - t0;
+    if (todo <= 0) return;
     aim(t0);
     fetch(0, emit);
     meet();  // sP; the tiles of an earlier run
-    for (int stage = 0; t0 < t1; t0 += TT, stage ^= 1) {
+    for (int stage = 0; todo > 0; todo -= TT, stage ^= 1) {
       const T* sX = reinterpret_cast<const T*>(smem + K::oX + stage * K::kStage);
       const T* own = sX + te * CB + ce;
       const T* sB = sX + 3 * TT * CB;
@@ -447,8 +449,8 @@ __global__ void __launch_bounds__(NT) scan_tiles_kernel(TileArgs q) {
         }
       }
       meet();
-      if (t0 + TT < t1) fetch(stage ^ 1, emit);
-      const int live = min_i(len - t0, TT);
+      if (todo > TT) fetch(stage ^ 1, emit);
+      const int live = min_i(todo, TT);
       // Software pipeline: while token t is accumulated, the decays of t + 1 are
       // computed (the exponentials' pipe is the scarce one) and the operands of
       // t + 2 read. Reads past the tile wrap around; nothing uses them.
@@ -560,7 +562,7 @@ __global__ void __launch_bounds__(NT) scan_tiles_kernel(TileArgs q) {
   if constexpr (CLUSTER) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
-    const int64_t each = ((int64_t)(len + TT - 1) / TT + q.parts - 1) / q.parts * TT;
+    const int64_t each = (((int64_t)len + TT - 1) / TT + q.parts - 1) / q.parts * TT;
     const int b0 = (int)(part * each < len ? part * each : len);
     const int b1 = (int)(b0 + each < len ? b0 + each : len);
     f32x2 start[NP][NS];
