@@ -15,6 +15,17 @@ BF, FH, F32 = torch.bfloat16, torch.float16, torch.float32
 NAMES = ("x", "dt", "A", "B", "C")
 
 
+def _inputs(cuda, lead, D, N, G, dtype, seed=0):
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, device=cuda)  # noqa: E731
+    return dict(x=r(*lead, D).to(dtype), dt=r(*lead, D).to(dtype), A=-torch.exp(r(D, N)), B=r(*lead, G, N).to(dtype),
+                C=r(*lead, G, N).to(dtype), D=r(D), z=r(*lead, D).to(dtype), dt_bias=r(D) - 4)
+
+
+def _call(fn, a, *state, **more):
+    return fn(*[a[k] for k in NAMES], *state, D=a["D"], z=a["z"], dt_bias=a["dt_bias"], **more)
+
+
 @pytest.mark.parametrize("T", [2 ** 26 + 7, 2 ** 31 - 1])
 def test_scan_longest_token_axis(cuda, T):
     """One channel of as many tokens as an int32 counts, the inputs repeated by
@@ -29,3 +40,48 @@ def test_scan_longest_token_axis(cuda, T):
     rest = o[0, 60:, 0]  # e^-30 of the empty start
     assert rest.min() == rest.max() and abs(rest[0].item() - 8 * h) <= (2.0 ** -8 + 2.0 ** -19) * 8 * h
     assert abs(o[0, 0, 0].item() - 4) <= 2.0 ** -8 * 4
+
+
+SHAPES = [(2, 5, 40, 16, 2), (160, 2, 1000, 16, 2),  # steps, one and four channels a thread
+          (2, 50, 40, 16, 2), (1, 60, 24, 128, 2),   # prompts
+          (64, 20, 2048, 16, 2),                     # many of them
+          (1, 2100, 40, 16, 2), (1, 1100, 8, 64, 2)]  # few long ones, split in time
+
+
+@pytest.mark.parametrize("B,T,D,N,G", SHAPES)
+@pytest.mark.parametrize("what", ["x", "dt", "A", "B", "C", "D", "z", "dt_bias", "state"])
+def test_scan_keeps_nan(cuda, B, T, D, N, G, what):
+    """A NaN in any input reaches what the formula makes of it, and nothing else."""
+    a = _inputs(cuda, (B, T), D, N, G, F32, seed=T)
+    h0 = torch.randn(B, D, N, device=cuda)
+    o, ht = _call(wk.selective_scan, a, initial_state=h0, output_final_state=True)
+    bad, g0, b, t, d, n = dict(a), h0.clone(), B - 1, T // 2, D // 2 + 1, N - 2
+    g = d // (D // G)
+    at = {"x": (b, t, d), "dt": (b, t, d), "z": (b, t, d), "A": (d, n), "B": (b, t, g, n), "C": (b, t, g, n), "D": (d,),
+          "dt_bias": (d,), "state": (b, d, n)}[what]
+    if what == "state":
+        g0[at] = float("nan")
+    else:
+        bad[what] = a[what].clone()
+        bad[what][at] = float("nan")
+    o2, ht2 = _call(wk.selective_scan, bad, initial_state=g0, output_final_state=True)
+    mo, mh = torch.zeros_like(o, dtype=torch.bool), torch.zeros_like(ht, dtype=torch.bool)
+    lo, hi = g * (D // G), (g + 1) * (D // G)
+    if what in ("x", "dt"):
+        mo[b, t:, d] = mh[b, d] = True
+    elif what == "A":
+        mo[:, :, d] = mh[:, d, n] = True
+    elif what == "B":
+        mo[b, t:, lo:hi] = mh[b, lo:hi, n] = True
+    elif what == "C":
+        mo[b, t, lo:hi] = True
+    elif what == "z":
+        mo[b, t, d] = True
+    elif what == "D":
+        mo[:, :, d] = True
+    elif what == "dt_bias":
+        mo[:, :, d] = mh[:, d] = True
+    else:
+        mo[b, :, d] = mh[b, d, n] = True
+    assert torch.equal(o2.isnan(), mo) and torch.equal(ht2.isnan(), mh)
+    assert torch.equal(o2[~mo], o[~mo]) and torch.equal(ht2[~mh], ht[~mh])

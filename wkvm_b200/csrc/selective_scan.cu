@@ -46,9 +46,13 @@ struct ScanArgs {
 // ---------------------------------------------------------------------------
 constexpr int kRowThreads = 128;
 
-// A as a power of two's exponent; finite, so that a step of zero keeps the
-// state even where A is -inf.
-__device__ __forceinline__ float scaled(float a) { return fmaxf(a * kLog2e, -FLT_MAX); }
+// A as a power of two's exponent; -FLT_MAX for -inf, so that a step of zero
+// keeps the state there too. NaN stays NaN (fmaxf would drop it).
+__device__ __forceinline__ float scaled(float a) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a * kLog2e), "f"(-FLT_MAX));
+  return r;
+}
 
 template <typename T, int N, int J>
 __global__ void __launch_bounds__(kRowThreads, 8) scan_rows_kernel(ScanArgs p) {
