@@ -85,3 +85,32 @@ def test_scan_keeps_nan(cuda, B, T, D, N, G, what):
         mo[b, :, d] = mh[b, d, n] = True
     assert torch.equal(o2.isnan(), mo) and torch.equal(ht2.isnan(), mh)
     assert torch.equal(o2[~mo], o[~mo]) and torch.equal(ht2[~mh], ht[~mh])
+
+
+@pytest.mark.parametrize("cu", [[0, 50, 10, 40], [0, 50, 60, -2, 1], [60, 100, 0, 40], [40, 100, 35, 38], [0, 33, 500, 70, 90],
+                                [5, 5, 64, 3, 3, 5]])
+@pytest.mark.parametrize("D", [40, 1032])
+def test_conv_offsets_out_of_order(cuda, cu, D):
+    """Sequences between offsets that descend or leave the axis are skipped;
+    every other one is computed, wherever it stands."""
+    T, W = 100, 4
+    x, w = torch.randn(1, T, D, device=cuda).to(BF), torch.randn(D, W, device=cuda).to(BF)
+    n = len(cu) - 1
+    bank = torch.randn(1, n + 1, W - 1, D, device=cuda).to(BF)
+    start, o = bank.clone(), torch.full_like(x, float("nan"))
+    wk.short_conv_prefill_slots(x, w, bank, 0, list(range(1, n + 1)), activation="silu",
+                                cu_seqlens=torch.tensor(cu, device=cuda), out=o)
+    with pytest.raises(_lib.WkvmError, match="INVALID_ARG"):
+        ops.check_device_status(cuda)
+    ok = [i for i in range(n) if 0 <= cu[i] <= cu[i + 1] <= T]
+    cover = torch.zeros(T, dtype=torch.int64)
+    for i in ok:
+        cover[cu[i]:cu[i + 1]] += 1
+    assert torch.equal(o[0].isnan().all(1).cpu(), cover == 0) and torch.equal(o[0].isnan().any(1).cpu(), cover == 0)
+    ref = start.clone()
+    for i in ok:
+        s = slice(cu[i], cu[i + 1])
+        want = wk.short_conv_prefill_slots(x[:, s], w, ref, 0, [i + 1], activation="silu")
+        one = (cover[s] == 1).to(cuda)  # tokens of two sequences may hold either's
+        assert torch.equal(o[0, s][one], want[0][one])
+    assert torch.equal(bank, ref)

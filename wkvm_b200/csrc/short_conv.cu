@@ -195,19 +195,26 @@ __global__ void __launch_bounds__(kThreads) short_conv_kernel(ConvArgs p) {
   const int c = ((int)(blk % cblocks) * kThreads + threadIdx.x) * V;
   const int64_t total = p.seqs.cu ? p.seqs.T : (int64_t)p.seqs.nseq * p.seqs.T;
   const int64_t t1 = t0 + kTile < total ? t0 + kTile : total;
-  // first sequence that ends past t0, found by the whole warp
-  int n = 0;
+  // the first sequence that ends past t0 and the last that begins before t1,
+  // found by the whole warp; offsets that descend leave others between them,
+  // which the loop skips
+  int n = 0, last = 0;
   if (p.seqs.cu) {
-    for (int i = threadIdx.x & 31; i < p.seqs.nseq; i += 32) n += p.seqs.cu[i + 1] <= t0;
-    n = __reduce_add_sync(0xffffffffu, n);
+    n = p.seqs.nseq;
+    for (int i = threadIdx.x & 31; i < p.seqs.nseq; i += 32) {
+      if (p.seqs.cu[i + 1] > t0) n = min(n, i);
+      if (p.seqs.cu[i] < t1) last = i;
+    }
+    n = __reduce_min_sync(0xffffffffu, n);
+    last = __reduce_max_sync(0xffffffffu, last);
   } else {
     n = (int)(t0 / p.seqs.T);
+    last = (int)((t1 - 1) / p.seqs.T);
   }
   if (c >= p.D) return;
   load_weights(c);
-  for (; n < p.seqs.nseq; ++n) {
+  for (; n <= last; ++n) {
     const SeqSpan sp = seq_span(p.seqs, n);
-    if (sp.bos >= t1) break;
     int64_t row;
     if (!sp.ok || !state_row(p.ids, p.num_slots, n, &row)) continue;
     const int64_t ta = t0 - sp.bos > p.head ? t0 - sp.bos : p.head;  // tokens of the sequence
