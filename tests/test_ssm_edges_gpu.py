@@ -114,3 +114,26 @@ def test_conv_offsets_out_of_order(cuda, cu, D):
         one = (cover[s] == 1).to(cuda)  # tokens of two sequences may hold either's
         assert torch.equal(o[0, s][one], want[0][one])
     assert torch.equal(bank, ref)
+
+
+@pytest.mark.parametrize("D,N", [(40, 16), (8, 64)])
+def test_scan_states_that_grow_between_parts(cuda, D, N):
+    """Without softplus steps may have any sign. Over a part of a long row a
+    state may grow by more than fp32's range: from nothing it stays nothing,
+    from a small value it is what the tokens one by one give."""
+    T = 2304
+    a = _inputs(cuda, (1, T), D, N, 1, F32, seed=N)
+    a["A"] = torch.ones(D, N, device=cuda)
+    a["dt_bias"] = None
+    sign = torch.where(torch.arange(T, device=cuda) // 144 % 2 == 0, 1.0, -1.0)
+    a["dt"] = (0.68 * sign)[None, :, None].expand(1, T, D).contiguous()  # e^98 up, e^98 down
+    a["x"] = torch.zeros_like(a["x"])
+    h0 = torch.zeros(1, D, N, device=cuda)
+    h0[:, ::2] = 1e-20 * (1 + torch.rand(1, (D + 1) // 2, N, device=cuda))
+    o, ht = _call(wk.selective_scan, a, dt_softplus=False, initial_state=h0, output_final_state=True)
+    ro, tol, rh, htol = ssm_ref.scan(*[a[k] for k in NAMES], a["D"], a["z"], None, False, h0)
+    assert bool(o.isfinite().all()) and not o[..., 1::2].any() and not ht[:, 1::2].any()
+    # a part's decay is the exponential of a sum of 144 steps, each rounded once:
+    # 144 x 2^-24 of a sum of 98 at most, that is 2^-10.2, sixteen parts
+    ssm_ref.check(o, ro, tol + 2.0 ** -6 * ro.abs(), "o")
+    ssm_ref.check(ht, rh, htol + 2.0 ** -6 * rh.abs(), "state")

@@ -54,6 +54,16 @@ __device__ __forceinline__ float scaled(float a) {
   return r;
 }
 
+// 2^e h + y for the decay 2^e over many tokens. Steps without softplus may have
+// any sign, so 2^e may leave fp32's range on either side where 2^e h does not:
+// then half of e at a time, and a state of nothing stays nothing.
+__device__ __forceinline__ float decayed(float e, float h, float y) {
+  if (fabsf(e) <= 126.0f) return fmaf(ex2(e), h, y);
+  if (h == 0.0f && e == e) return y;
+  const float f = ex2(0.5f * e);
+  return fmaf(h * f, f, y);
+}
+
 template <typename T, int N, int J>
 __global__ void __launch_bounds__(kRowThreads, 8) scan_rows_kernel(ScanArgs p) {
   constexpr int LPC = N / 4;  // lanes of a channel
@@ -594,7 +604,8 @@ __global__ void __launch_bounds__(NT) scan_tiles_kernel(TileArgs q) {
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
           const float2 e = unpack2(mul2(a[j][i], sum));
-          start[j][i] = fma2(pack2(ex2(e.x), ex2(e.y)), start[j][i], peer[(j * NS + i) * NT]);
+          const float2 x = unpack2(start[j][i]), y = unpack2(peer[(j * NS + i) * NT]);
+          start[j][i] = pack2(decayed(e.x, x.x, y.x), decayed(e.y, x.y, y.y));
         }
       }
     }
