@@ -89,3 +89,28 @@ def test_threads_with_vocabularies_of_their_own(cuda):
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("V", [900, 3000, 40000])
+def test_temperature_without_limit_and_min_p(cuda, V):
+    """At an infinite temperature every weight is 1, and so at least min_p."""
+    x, u = _logits(6, V, V, cuda)
+    x[:, V // 2:] = -INF
+    inf = torch.full((6,), INF, device=cuda)
+    for s in (dict(min_p=1.0), dict(min_p=0.5), dict(min_p=1.0, top_p=0.5), dict(min_p=1.0, top_k=V)):
+        n = V // 2
+        if "top_p" in s:  # the largest half of them
+            tok, lp = wk.sample_tokens(x, u, temperature=inf, **s)
+            kept = math.ceil(n / 2)
+            rank = (x > x.gather(1, tok[:, None])).sum(1)
+            assert bool((rank < kept).all())
+        else:
+            kept = n
+            tok, lp = wk.sample_tokens(x, u, temperature=inf, **s)
+            assert torch.equal(tok, (u.double() * n).long())
+        assert bool(((lp + math.log(kept)).abs() < 1e-6).all())
+    for t in (1e30, 1e18):  # weights round to 1
+        for s in (dict(min_p=1.0), dict(min_p=0.5), dict()):
+            tok, lp = wk.sample_tokens(x, u, temperature=t, **s)
+            want, wlp = _want(x, u, temperature=t, **s)
+            assert tok.tolist() == want.tolist() and _near(lp, wlp, V)

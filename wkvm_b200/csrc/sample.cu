@@ -802,9 +802,10 @@ __global__ void __launch_bounds__(kNT, 2) sample_kernel(SampleArgs p) {
 
   // ---- draw from the whole row: masses of contiguous blocks, one per warp
   const int per = p.slice / kWarps, i0 = r.warp * per;
-  // logits this low have w < mp for certain
+  // logits this low have w < mp for certain, as w is computed: 1e-9 of the
+  // exponent covers its error, at temperatures where every weight rounds to 1 too
   const float low = mp > 0.0 && !r.flat
-                        ? (float)(r.top + log2(mp) / r.c * 1.0001 - fabs((double)r.top) * 3e-7) : -INFINITY;
+                        ? (float)(r.top + (log2(mp) - 1e-9) / r.c * 1.0001 - fabs((double)r.top) * 3e-7) : -INFINITY;
   auto may = [&](float l, int i) { return (l >= low || l == r.top) && r.kept(l, r.base + i); };
   auto share = [&](float l, double w) { return w >= mp || l == r.top ? r.units(w) : 0; };
   u64 sum = 0;
