@@ -1,0 +1,45 @@
+"""Calls of the selective state space operators and of sampling that are
+refused on the host, and the host's checks of tokens (no GPU, nothing launched)."""
+
+import math
+
+import pytest
+import torch
+
+import wkvm_b200 as wk
+
+
+@pytest.fixture
+def anywhere(monkeypatch):
+    """The checks behind the one for CUDA tensors; a launch is recorded instead."""
+    from wkvm_b200 import ops
+    calls = []
+    monkeypatch.setattr(ops, "_require_cuda", lambda *t: None)
+    monkeypatch.setattr(ops, "_launch", lambda name, idx, *args: calls.append((name, args)))
+    return calls
+
+
+def _top_k0(call):
+    return call[1][8]  # of wkvm_sample_tokens: the scalar beside the device array
+
+
+def test_top_k_is_a_whole_number(anywhere):
+    x, u = torch.zeros(3, 9), torch.zeros(3)
+    for k in (0.5, 2.7, math.inf):
+        with pytest.raises(ValueError, match="top_k must be a whole number"):
+            wk.sample_tokens(x, u, top_k=k)
+    assert not anywhere
+    for k, want in ((4, 4), (4.0, 4), (0, 0), (10 ** 12, 9)):
+        wk.sample_tokens(x, u, top_k=k)
+        assert _top_k0(anywhere[-1]) == want
+
+
+def test_top_k_tensors_become_whole_numbers():
+    """Per-row values of any type reach the kernel as int32; a fraction never as the 0 that keeps everything."""
+    from wkvm_b200.sampling import _setting
+    x = torch.zeros(4, 9)
+    for value, want in ((torch.tensor([0.0, 0.5, 2.7, 1e12]), [0, 1, 3, 1 << 30]),
+                        (torch.tensor([-3, 0, 7, 1 << 40]), [0, 0, 7, 1 << 30]),
+                        (torch.tensor(0.25, dtype=torch.float64), [1] * 4)):
+        got, scalar = _setting("top_k", value, 4, torch.int32, x)
+        assert got.dtype is torch.int32 and got.tolist() == want and scalar == 0

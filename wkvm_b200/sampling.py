@@ -16,6 +16,10 @@ def _setting(name: str, value, rows: int, dtype: torch.dtype, logits: torch.Tens
     if not isinstance(value, torch.Tensor):
         if value is None or not value >= 0:
             raise ValueError(f"{name} must be >= 0, not {value!r}")
+        if dtype is torch.int32:
+            if value == float("inf") or value != int(value):
+                raise ValueError(f"{name} must be a whole number, not {value!r}")
+            value = int(value)
         return None, value
     if value.dim() == 0:
         value = value.expand(rows)
@@ -24,7 +28,8 @@ def _setting(name: str, value, rows: int, dtype: torch.dtype, logits: torch.Tens
     if value.dtype is dtype and value.get_device() == logits.get_device() and value.is_contiguous():
         return value, 0
     if dtype is torch.int32 and value.dtype is not torch.int32:
-        value = value.clamp(0, (1 << 31) - 1)
+        # a fraction is rounded up, so that it never becomes the 0 that keeps all
+        value = (value.ceil() if value.is_floating_point() else value).clamp(0, 1 << 30)
     return value.to(device=logits.device, dtype=dtype).contiguous(), 0
 
 
@@ -36,9 +41,9 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     logprobs fp32 [B]), the log-probabilities under the filtered distribution.
 
     With w_i = exp((l_i - max l) / temperature): ``top_k`` keeps the k largest
-    logits (0: all); ``top_p`` keeps, of those in descending order, the
-    shortest prefix that holds at least that share of their mass (1: all);
-    ``min_p`` keeps, of those, w_i >= min_p (0: all). The token is the first
+    logits (0: all; a whole number, fractions in a tensor are rounded up);
+    ``top_p`` keeps, of those in descending order, the shortest prefix that
+    holds at least that share of their mass (1: all); ``min_p`` keeps, of those, w_i >= min_p (0: all). The token is the first
     kept id whose running mass, over ascending ids, exceeds u times the mass
     kept. Ties go to the lowest ids; temperature 0 is greedy. -inf (and NaN)
     logits are never chosen; a row of nothing else gives token -1 and
@@ -73,6 +78,6 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     tokens, logprobs = torch.empty_like(u, dtype=torch.int64), torch.empty_like(u)
     p = _ops._ptr
     _ops._launch("wkvm_sample_tokens", idx, logits.data_ptr(), stride, u.data_ptr(), p(temp), p(k), p(tp), p(mp),
-                 float(temp0), min(int(k0), V), float(tp0), float(mp0), tokens.data_ptr(), logprobs.data_ptr(), B, V,
+                 float(temp0), min(k0, V), float(tp0), float(mp0), tokens.data_ptr(), logprobs.data_ptr(), B, V,
                  _ops._DTYPES[logits.dtype])
     return tokens, logprobs
