@@ -43,3 +43,17 @@ def test_top_k_tensors_become_whole_numbers():
                         (torch.tensor(0.25, dtype=torch.float64), [1] * 4)):
         got, scalar = _setting("top_k", value, 4, torch.int32, x)
         assert got.dtype is torch.int32 and got.tolist() == want and scalar == 0
+
+
+def test_sampling_refuses_inputs_that_ask_for_gradients(anywhere):
+    x, u = torch.zeros(3, 9), torch.zeros(3)
+    t = lambda: torch.ones(3, requires_grad=True)  # noqa: E731
+    for change in (dict(logits=torch.zeros(3, 9, requires_grad=True)), dict(u=t()), dict(temperature=t()),
+                   dict(top_p=t()), dict(min_p=t())):
+        kw = dict(logits=x, u=u) | change
+        with pytest.raises(RuntimeError, match="no backward"):
+            wk.sample_tokens(**kw)
+        assert not anywhere
+        with torch.no_grad():
+            wk.sample_tokens(**kw)
+        assert anywhere.pop()

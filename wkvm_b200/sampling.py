@@ -48,12 +48,18 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     kept. Ties go to the lowest ids; temperature 0 is greedy. -inf (and NaN)
     logits are never chosen; a row of nothing else gives token -1 and
     log-probability -inf. The same inputs give the same tokens on every run,
-    eagerly and in a captured graph."""
+    eagerly and in a captured graph. Forward only: inputs that ask for
+    gradients are refused."""
     idx = logits.get_device()
     if idx < 0 or u.get_device() != idx:
         _ops._require_cuda(logits, u)
         if u.device != logits.device:
             raise ValueError(f"u must be on {logits.device}, not {u.device}")
+    if torch.is_grad_enabled():
+        for t in (logits, u, temperature, top_p, min_p):
+            if isinstance(t, torch.Tensor) and t.requires_grad:
+                raise RuntimeError("this operator has no backward pass: call it under torch.no_grad() or "
+                                   "with detached tensors")
     if logits.dim() != 2:
         raise ValueError(f"logits must be [B, V], not {tuple(logits.shape)}")
     if logits.dtype not in _ops._DTYPES:
