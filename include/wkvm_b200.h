@@ -367,7 +367,7 @@ int wkvm_selective_scan_slots(
     int32_t D, int32_t N, int32_t G, int32_t softplus, int32_t dtype,
     int32_t* status, wkvm_stream_t stream);
 
-enum { WKVM_SAMPLE_MAX_VOCAB = 1 << 30 };
+enum { WKVM_SAMPLE_MAX_VOCAB = 1 << 20 };
 
 /* Chooses one token for each of B rows of V logits (row_stride elements
  * apart) from a given uniform number u[b] in [0, 1). With m the row's
@@ -381,9 +381,13 @@ enum { WKVM_SAMPLE_MAX_VOCAB = 1 << 30 };
  * Ties go to the lowest ids. temperature <= 0 is greedy: the largest logit,
  * logprob 0. -inf and NaN logits are never chosen, +inf ones share the whole
  * mass, and a row with nothing to choose gives token -1 and logprob -inf.
- * Masses are rounded to V 2^-46 (65,536 logits; less for fewer) of the largest
- * weight and summed exactly: the same inputs give the same token on every run. V is at most WKVM_SAMPLE_MAX_VOCAB. Each setting is a device array [B], or NULL
- * and the scalar beside it holds for every row. */
+ * Weights are rounded to units of 2^-s of the largest, s = min(52, 62 -
+ * ceil(log2 V)), and summed exactly: the same inputs give the same token on
+ * every run. A running mass is off by V 2^-(s+1) at most (2^-31 at V = 65,536),
+ * and a weight of less than half a unit is never drawn, by u = 0 neither. V is
+ * at most WKVM_SAMPLE_MAX_VOCAB, where that is 2^-23, two steps of an fp32 u.
+ * Each setting is a device array [B], or NULL and the scalar beside it holds
+ * for every row. */
 int wkvm_sample_tokens(
     const void* logits, int64_t row_stride, const float* u, const float* temperature,
     const int32_t* top_k, const float* top_p, const float* min_p, float temperature0,

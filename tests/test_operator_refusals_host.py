@@ -1,6 +1,7 @@
 """Calls of the selective state space operators and of sampling that are
 refused on the host, and the host's checks of tokens (no GPU, nothing launched)."""
 
+import ctypes
 import math
 
 import pytest
@@ -57,3 +58,15 @@ def test_sampling_refuses_inputs_that_ask_for_gradients(anywhere):
         with torch.no_grad():
             wk.sample_tokens(**kw)
         assert anywhere.pop()
+
+
+def test_vocabularies_beyond_the_masses_resolution(anywhere):
+    """Past 2^20 logits the masses' rounding would exceed two steps of an fp32 u."""
+    x = torch.zeros(1, 1).expand(1, (1 << 20) + 1)
+    with pytest.raises(ValueError, match="a vocabulary of 1048577 is not supported"):
+        wk.sample_tokens(x, torch.zeros(1))
+    assert not anywhere
+    from wkvm_b200 import _lib, build
+    build.build()
+    p, f, n = ctypes.c_void_p(4096), ctypes.c_float, None
+    assert _lib.load().wkvm_sample_tokens(p, 8, p, n, n, n, n, f(1), 0, f(1), f(0), p, p, 1, (1 << 20) + 1, 1, n, n) == -2

@@ -114,3 +114,29 @@ def test_temperature_without_limit_and_min_p(cuda, V):
             tok, lp = wk.sample_tokens(x, u, temperature=t, **s)
             want, wlp = _want(x, u, temperature=t, **s)
             assert tok.tolist() == want.tolist() and _near(lp, wlp, V)
+
+
+def test_weights_below_half_a_unit_are_never_drawn(cuda):
+    """Weights are rounded to units of 2^-s: the smallest number draws the first id with one."""
+    V = 5000  # s = 62 - 13 = 49
+    x = torch.full((3, V), -200.0, device=cuda)  # e^-200: no unit
+    x[:, 4000] = 0.0
+    x[1, 3000] = -48 * math.log(2)               # two units
+    x[2, 3000] = -51 * math.log(2)               # a quarter of one
+    zero = torch.zeros(3, device=cuda)
+    for s in (dict(), dict(top_k=100), dict(top_p=1 - 2.0 ** -24)):
+        tok, lp = wk.sample_tokens(x, zero, **s)
+        assert tok.tolist()[::2] == [4000, 4000] and bool((lp[::2] == 0).all())
+        if "top_p" not in s:
+            assert tok[1] == 3000 and abs(lp[1].item() + 48 * math.log(2)) < 1e-5
+
+
+def test_largest_vocabulary(cuda):
+    """2^20 logits: a border moves by V 2^-43 = 2^-23 of the largest weight at most."""
+    V = wk.sampling.MAX_VOCAB
+    assert V == 1 << 20
+    x, u = _logits(3, V, 1, cuda, BF)
+    for s in (dict(), dict(top_p=0.9), dict(top_k=100, top_p=0.9), dict(min_p=0.05)):
+        tok, lp = wk.sample_tokens(x, u, **s)
+        want, wlp = _want(x, u, **s)
+        assert tok.tolist() == want.tolist() and _near(lp, wlp, V)

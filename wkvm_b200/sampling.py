@@ -8,7 +8,8 @@ from . import _lib
 from . import ops as _ops
 
 
-MAX_VOCAB = 1 << 30  # WKVM_SAMPLE_MAX_VOCAB
+# WKVM_SAMPLE_MAX_VOCAB: there the masses' rounding reaches two steps of an fp32 u
+MAX_VOCAB = 1 << 20
 
 
 def _setting(name: str, value, rows: int, dtype: torch.dtype, logits: torch.Tensor):
@@ -45,7 +46,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     ``top_p`` keeps, of those in descending order, the shortest prefix that
     holds at least that share of their mass (1: all); ``min_p`` keeps, of those, w_i >= min_p (0: all). The token is the first
     kept id whose running mass, over ascending ids, exceeds u times the mass
-    kept. Ties go to the lowest ids; temperature 0 is greedy. -inf (and NaN)
+    kept (masses hold 2^-46 of the largest weight at 65,536 logits; less is
+    never drawn). Ties go to the lowest ids; temperature 0 is greedy. -inf (and NaN)
     logits are never chosen; a row of nothing else gives token -1 and
     log-probability -inf. The same inputs give the same tokens on every run,
     eagerly and in a captured graph. Forward only: inputs that ask for
