@@ -70,3 +70,46 @@ def test_vocabularies_beyond_the_masses_resolution(anywhere):
     build.build()
     p, f, n = ctypes.c_void_p(4096), ctypes.c_float, None
     assert _lib.load().wkvm_sample_tokens(p, 8, p, n, n, n, n, f(1), 0, f(1), f(0), p, p, 1, (1 << 20) + 1, 1, n, n) == -2
+
+
+class _Model:
+    """Stands in for a causal language model; a forward pass would be recorded."""
+
+    def __init__(self, vocab):
+        self.table, self.seen = torch.nn.Embedding(vocab, 2), []
+
+    def get_input_embeddings(self):
+        return self.table
+
+    def __call__(self, input_ids, **kw):
+        self.seen.append(input_ids)
+        raise AssertionError("the model was called")
+
+
+class _Bank:
+    device, num_slots = torch.device("cpu"), 4
+
+    def gather_cache(self, slot_batch):
+        return None
+
+
+@pytest.mark.parametrize("tokens", [[3, -1], [50, 7], [-1, 2 ** 40]])
+def test_tokens_outside_the_vocabulary_never_reach_the_model(tokens):
+    """-1 is what sampling gives for a row with nothing to choose; the
+    embedding's lookup would fault on the device."""
+    from wkvm_b200.graph import GraphedDecode
+    from wkvm_b200.runner import RWKV7Runner, checked_tokens
+    model, batch = _Model(50), [{"wkv": 1, "shift": 1}, {"wkv": 2, "shift": 2}]
+    runner = RWKV7Runner(model, _Bank())
+    graphed = GraphedDecode.__new__(GraphedDecode)  # a captured step, without its graph
+    graphed.runner, graphed.batch_size = runner, 2
+    for call in (lambda: runner.decode_step(batch, tokens), lambda: runner.prefill(tokens, batch[0]),
+                 lambda: runner.sample_step(batch, tokens, torch.zeros(2)), lambda: graphed.decode_step(batch, tokens),
+                 lambda: graphed.sample_step(batch, tokens, torch.zeros(2))):
+        with pytest.raises(ValueError, match="leave the vocabulary of 50"):
+            call()
+    assert not model.seen
+    with pytest.raises(AssertionError, match="the model was called"):
+        runner.decode_step(batch, [0, 49])
+    assert model.seen[0].tolist() == [[0], [49]]
+    assert checked_tokens([], model).numel() == 0

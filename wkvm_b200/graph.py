@@ -25,6 +25,7 @@ from __future__ import annotations
 import torch
 
 from . import fla_compat, ops
+from .runner import checked_tokens
 from .sampling import sample_tokens
 
 
@@ -94,6 +95,7 @@ class GraphedDecode:
         if not 0 < n <= self.batch_size:
             raise ValueError(f"batch of {n} rows for a graph of {self.batch_size}")
         bank = self.runner.bank
+        last = checked_tokens(last_tokens, self.runner.model)
         wkv = [int(s["wkv"]) for s in slot_batch]
         shift = [int(s["shift"]) for s in slot_batch]
         # range and duplicate checks on the host (the padding rows are slot 0)
@@ -103,7 +105,7 @@ class GraphedDecode:
         if self._staged is not None:
             self._staged.synchronize()  # the previous call's copy has read h
         h.zero_()
-        h[0, :n] = torch.tensor(last_tokens)
+        h[0, :n] = last
         h[1, :n] = torch.tensor(wkv)
         h[2, :n] = torch.tensor(shift)
         dev = bank.device

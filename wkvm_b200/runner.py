@@ -24,6 +24,20 @@ from . import fla_compat
 from .sampling import sample_tokens
 
 
+def checked_tokens(tokens, model) -> torch.Tensor:
+    """Token ids as an int64 host tensor. Ids outside the model's embedding are
+    refused: its lookup would fault on the device. (-1 is what sampling gives
+    for a row with nothing to choose.)"""
+    ids = torch.tensor(tokens, dtype=torch.long)
+    if ids.numel():
+        least, most = (int(v) for v in torch.aminmax(ids))
+        table = getattr(model.get_input_embeddings(), "weight", None) if hasattr(model, "get_input_embeddings") else None
+        if least < 0 or (table is not None and most >= table.shape[0]):
+            limit = "" if table is None else f" of {table.shape[0]}"
+            raise ValueError(f"token ids {least} to {most} leave the vocabulary{limit}")
+    return ids
+
+
 class RWKV7Runner:
     """Prefill / decode over slots of an :class:`~wkvm_b200.state.RWKV7StateBank`."""
 
@@ -45,7 +59,7 @@ class RWKV7Runner:
         logits as fp32 ``[vocab]``."""
         if not token_ids:
             raise ValueError("empty prompt")
-        ids = torch.tensor(token_ids, dtype=torch.long, device=self.device)
+        ids = checked_tokens(token_ids, self.model).to(self.device)
         logits = None
         for start in range(0, len(token_ids), self.prefill_chunk):
             piece = ids[start:start + self.prefill_chunk].unsqueeze(0)
@@ -62,7 +76,7 @@ class RWKV7Runner:
         next-token logits as fp32 ``[batch, vocab]``."""
         if len(slot_batch) != len(last_tokens):
             raise ValueError("slot_batch and last_tokens length mismatch")
-        ids = torch.tensor(last_tokens, dtype=torch.long, device=self.device)
+        ids = checked_tokens(last_tokens, self.model).to(self.device)
         if fla_compat.fused_installed():
             # shift family in the bank too: the fused prologues read and
             # write it in place, so there is nothing to commit afterwards
@@ -85,6 +99,7 @@ class RWKV7Runner:
         """:meth:`decode_step` and the choice of the next tokens from the
         uniform numbers ``u`` [batch] (:func:`wkvm_b200.sample_tokens`, whose
         settings are numbers or one value per row). Returns (tokens int64
-        [batch], log-probabilities fp32 [batch]) on the device."""
+        [batch], log-probabilities fp32 [batch]) on the device. A row whose
+        logits are all -inf or NaN gets token -1, which the next step refuses."""
         return sample_tokens(self.decode_step(slot_batch, last_tokens), u, temperature=temperature, top_k=top_k,
                              top_p=top_p, min_p=min_p)
