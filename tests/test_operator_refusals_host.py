@@ -113,3 +113,18 @@ def test_tokens_outside_the_vocabulary_never_reach_the_model(tokens):
         runner.decode_step(batch, [0, 49])
     assert model.seen[0].tolist() == [[0], [49]]
     assert checked_tokens([], model).numel() == 0
+
+
+def test_sizes_beyond_32_bits_are_refused(anywhere):
+    """The kernels count in int32: a larger size would wrap in the call, to a smaller one that runs."""
+    big = (1 << 32) + 8
+    e = lambda *s: torch.empty(*s, device="meta")  # noqa: E731
+    for B, T, D in ((1, 1, big), (1, big, 8), (big, 1, 8)):
+        x, bc = e(B, T, D), e(B, T, 8)
+        with pytest.raises(ValueError, match="more than an int32 counts"):
+            wk.short_conv(x, e(D, 4))
+        with pytest.raises(ValueError, match="more than an int32 counts"):
+            wk.selective_scan(x, x, e(D, 8), bc, bc)
+    with pytest.raises(ValueError, match="more than an int32 counts"):
+        wk.sample_tokens(e(big, 1), e(big))
+    assert not anywhere

@@ -69,6 +69,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     B, V = logits.shape
     if V < 1 or V > MAX_VOCAB:
         raise ValueError(f"a vocabulary of {V} is not supported")
+    if B >= 1 << 31:
+        raise ValueError(f"{B} rows are more than an int32 counts")
     if u.dim() != 1 or u.shape[0] != B:
         raise ValueError(f"u must be [{B}], not {tuple(u.shape)}")
     temp, temp0 = _setting("temperature", temperature, B, torch.float32, logits)

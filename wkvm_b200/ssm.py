@@ -26,6 +26,7 @@ from . import ops as _ops
 
 _STATES = (8, 16, 32, 64, 128)
 _WIDTHS = (2, 3, 4)
+_INT32 = (1 << 31) - 1
 _ACTIVATIONS = {None: 0, "silu": 1, "swish": 1}
 _strides = struct.Struct("10q").pack  # the C call's array of ten int64
 
@@ -71,9 +72,9 @@ def _f32(t: torch.Tensor | None) -> torch.Tensor | None:
 
 def _sequences(x: torch.Tensor, cu_seqlens):
     """(number of sequences, tokens for the C call, cu_seqlens on the device)."""
-    B, T = x.shape[0], x.shape[1]
-    if T >= 1 << 31:
-        raise ValueError(f"{T} tokens are more than an int32 counts")
+    B, T, D = x.shape
+    if B > _INT32 or T > _INT32 or D > _INT32:
+        raise ValueError(f"a size of {(B, T, D)} is more than an int32 counts")
     if cu_seqlens is None:
         return B, T, None
     _ops._check_varlen(x, None, cu_seqlens)
