@@ -140,3 +140,13 @@ def test_largest_vocabulary(cuda):
         tok, lp = wk.sample_tokens(x, u, **s)
         want, wlp = _want(x, u, **s)
         assert tok.tolist() == want.tolist() and _near(lp, wlp, V)
+
+
+@pytest.mark.parametrize("s", [dict(), dict(top_k=9), dict(top_p=0.9), dict(min_p=0.01)], ids=str)
+def test_numbers_outside_their_range(cuda, s):
+    """Below 0 as 0, at or past 1 the last kept id with a mass, against the definition."""
+    x, _ = _logits(6, 2000, 4, cuda)
+    for u, like in ((-1.0, 0.0), (NAN, 0.0), (-INF, 0.0), (1.0, 1.0), (2.0, 1.0), (INF, 1.0)):
+        tok, lp = wk.sample_tokens(x, torch.full((6,), u, device=cuda), **s)
+        want, wlp = _want(x, torch.full((6,), like), **s)
+        assert tok.tolist() == want.tolist() and _near(lp, wlp, 2000)

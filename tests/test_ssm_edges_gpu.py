@@ -137,3 +137,53 @@ def test_scan_states_that_grow_between_parts(cuda, D, N):
     # 144 x 2^-24 of a sum of 98 at most, that is 2^-10.2, sixteen parts
     ssm_ref.check(o, ro, tol + 2.0 ** -6 * ro.abs(), "o")
     ssm_ref.check(ht, rh, htol + 2.0 ** -6 * rh.abs(), "state")
+
+
+# rows enough for four channels a thread (B D N >= 16 x 148 x 1024), with a
+# last block of channels that is not full and groups that end inside a block
+@pytest.mark.parametrize("dtype,B,D,N,G", [(BF, 160, 1002, 16, 3), (F32, 310, 1001, 8, 1), (FH, 304, 1002, 8, 6),
+                                           (BF, 80, 1001, 32, 7), (F32, 40, 990, 64, 10), (FH, 20, 1002, 128, 2),
+                                           (F32, 160, 1002, 16, 1)])
+@pytest.mark.parametrize("T", [1, 3, 8])
+def test_scan_steps_of_many_rows(cuda, dtype, B, D, N, G, T):
+    assert B * D * N >= 16 * 148 * 1024
+    a = _inputs(cuda, (B, T), D, N, G, dtype, seed=N + T)
+    bank = torch.randn(1, B + 3, D, N, device=cuda)
+    before = bank.clone()
+    ids = (1 + torch.randperm(B + 2, generator=torch.Generator().manual_seed(T))[:B]).tolist()
+    o = _call(wk.selective_scan_decode_slots, a, bank, 0, ids)
+    ro, tol, rh, htol = ssm_ref.scan(*[a[k] for k in NAMES], a["D"], a["z"], a["dt_bias"], True, before[0, ids])
+    ssm_ref.check(o, ro, tol, "o")
+    ssm_ref.check(bank[0, ids], rh, htol, "state")
+    rest = [i for i in range(B + 3) if i not in ids]
+    assert torch.equal(bank[0, rest], before[0, rest])
+    ops.check_device_status(cuda)
+
+
+@pytest.mark.parametrize("dtype,B,T,D,N,G", [(BF, 16, 19, 2050, 16, 2), (F32, 33, 9, 2001, 8, 3), (FH, 9, 33, 2004, 32, 4),
+                                             (F32, 9, 17, 1000, 64, 1), (BF, 5, 40, 1030, 128, 2), (F32, 17, 16, 2048, 16, 1)])
+def test_scan_prompts_of_many_rows(cuda, dtype, B, T, D, N, G):
+    """The wide launch shape (B D N >= 2048 x 256) against 64 bits."""
+    assert B * D * N >= 2048 * 256 and D % G == 0
+    a = _inputs(cuda, (B, T), D, N, G, dtype, seed=B)
+    h0 = torch.randn(B, D, N, device=cuda)
+    o, ht = _call(wk.selective_scan, a, initial_state=h0, output_final_state=True)
+    ro, tol, rh, htol = ssm_ref.scan(*[a[k] for k in NAMES], a["D"], a["z"], a["dt_bias"], True, h0)
+    ssm_ref.check(o, ro, tol, "o")
+    ssm_ref.check(ht, rh, htol, "state")
+
+
+@pytest.mark.parametrize("D,N", [(40, 16), (8, 64), (12, 128)])
+def test_scan_parts_join_without_loss(cuda, D, N):
+    """Steps of 1/4 add up exactly and slow decays carry states over every part
+    of a long row: the bounds of the tokens one by one hold as they are."""
+    T = 2100
+    a = _inputs(cuda, (1, T), D, N, 1, F32, seed=N)
+    a["dt"], a["dt_bias"] = torch.full_like(a["dt"], 0.25), None
+    a["A"] = -torch.exp(-7 * torch.rand(D, N, device=cuda))  # e-folds from 4 to 4,400 tokens
+    a["x"] = a["x"] * (torch.rand(1, T, 1, device=cuda) < 0.02)
+    h0 = 10 * torch.randn(1, D, N, device=cuda)
+    o, ht = _call(wk.selective_scan, a, dt_softplus=False, initial_state=h0, output_final_state=True)
+    ro, tol, rh, htol = ssm_ref.scan(*[a[k] for k in NAMES], a["D"], a["z"], None, False, h0)
+    ssm_ref.check(o, ro, tol, "o")
+    ssm_ref.check(ht, rh, htol, "state")
