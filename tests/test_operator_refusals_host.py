@@ -128,3 +128,28 @@ def test_sizes_beyond_32_bits_are_refused(anywhere):
     with pytest.raises(ValueError, match="more than an int32 counts"):
         wk.sample_tokens(e(big, 1), e(big))
     assert not anywhere
+
+
+def test_restored_host_copies_live_until_the_kernels_have_read_them(monkeypatch):
+    """The restore kernels read pinned memory directly, and its allocator does
+    not know: a copy freed ahead of the synchronise could be handed out again."""
+    import gc
+    import weakref
+
+    from wkvm_b200 import state
+    staged, read = [], []
+
+    class Stream:
+        def synchronize(self):
+            gc.collect()
+            read.append([r() is not None for r in staged])
+
+    monkeypatch.setattr(state, "_pinned", lambda t: t.clone())
+    monkeypatch.setattr(state.ops, "slot_restore", lambda fam, dim, ids, packed: staged.append(weakref.ref(packed)))
+    monkeypatch.setattr(state.torch.cuda, "current_stream", lambda dev: Stream())
+    bank = state.SSMStateBank(state.SSMStateLayout(2, 24, 8, 3, torch.float16), num_slots=3, device="cpu")
+    bank.restore([1, 2], {"ssm": torch.zeros(2, 2, 24, 8), "conv": torch.zeros(2, 2, 2, 24, dtype=torch.float16)})
+    lay = state.RWKV7StateLayout(n_layer=2, hidden_size=8, num_heads=1, head_dim=4, head_v_dim=4)
+    bank = state.RWKV7StateBank(lay, num_slots=3, device="cpu")
+    bank.restore({"wkv": 1, "shift": 1}, {"wkv": torch.zeros(2, 1, 4, 4), "shift": torch.zeros(2, 2, 8)})
+    assert read[0] == [True, True] and read[1][2:] == [True, True]

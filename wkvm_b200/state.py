@@ -183,10 +183,11 @@ class RWKV7StateBank:
 
     def restore(self, slots: SlotDict, tensors: Mapping[str, torch.Tensor]) -> None:
         """Inverse of :meth:`snapshot` (wkvm StateStore.load). Synchronises."""
-        wkv = tensors["wkv"].reshape(1, *tensors["wkv"].shape)
-        shift = tensors["shift"].reshape(1, *tensors["shift"].shape)
-        ops.slot_restore(self.wkv, 1, [int(slots["wkv"])], _pinned(wkv))
-        ops.slot_restore(self.shift, 2, [int(slots["shift"])], _pinned(shift))
+        # pinned copies stay alive until the kernels have read them
+        wkv = _pinned(tensors["wkv"].reshape(1, *tensors["wkv"].shape))
+        shift = _pinned(tensors["shift"].reshape(1, *tensors["shift"].shape))
+        ops.slot_restore(self.wkv, 1, [int(slots["wkv"])], wkv)
+        ops.slot_restore(self.shift, 2, [int(slots["shift"])], shift)
         torch.cuda.current_stream(self.device).synchronize()
 
     # -- migration --------------------------------------------------------
@@ -298,8 +299,9 @@ class SSMStateBank:
 
     def restore(self, slots: Sequence[int], tensors: Mapping[str, torch.Tensor]) -> None:
         """Inverse of :meth:`snapshot`. Synchronises."""
-        for name, dim in self.FAMILIES:
-            ops.slot_restore(getattr(self, name), dim, slots, _pinned(tensors[name]))
+        staged = [_pinned(tensors[name]) for name, _ in self.FAMILIES]  # alive until the kernels have read them
+        for (name, dim), t in zip(self.FAMILIES, staged):
+            ops.slot_restore(getattr(self, name), dim, slots, t)
         torch.cuda.current_stream(self.device).synchronize()
 
     def state_bytes(self) -> int:
