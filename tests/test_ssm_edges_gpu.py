@@ -187,3 +187,70 @@ def test_scan_parts_join_without_loss(cuda, D, N):
     ro, tol, rh, htol = ssm_ref.scan(*[a[k] for k in NAMES], a["D"], a["z"], None, False, h0)
     ssm_ref.check(o, ro, tol, "o")
     ssm_ref.check(ht, rh, htol, "state")
+
+
+@pytest.mark.parametrize("B,D,N", [(6, 96, 16), (300, 1024, 16)])
+def test_padded_batches(cuda, B, D, N):
+    """Rows padded with slot 0, as a graphed step pads them, share that row and change no other."""
+    a = _inputs(cuda, (B, 1), D, N, 1, BF)
+    w = torch.randn(D, 4, device=cuda).to(BF)
+    n = B // 2 + 1
+    ids = torch.zeros(B, dtype=torch.int32, device=cuda)
+    ids[:n] = 1 + torch.randperm(n, device=cuda)
+    conv, ssm = torch.randn(1, n + 2, 3, D, device=cuda).to(BF), torch.randn(1, n + 2, D, N, device=cuda)
+    conv2, ssm2 = conv.clone(), ssm.clone()
+    y = wk.short_conv_decode_slots(a["x"], w, conv, 0, ids)
+    o = _call(wk.selective_scan_decode_slots, a, ssm, 0, ids)
+    real = {k: v[:n] if k in ("x", "dt", "B", "C", "z") else v for k, v in a.items()}
+    y2 = wk.short_conv_decode_slots(real["x"], w, conv2, 0, ids[:n])
+    o2 = _call(wk.selective_scan_decode_slots, real, ssm2, 0, ids[:n])
+    assert torch.equal(y[:n], y2) and torch.equal(o[:n], o2)
+    assert torch.equal(conv[:, 1:], conv2[:, 1:]) and torch.equal(ssm[:, 1:], ssm2[:, 1:])
+    ops.check_device_status(cuda)
+
+
+def test_captured_prompts(cuda):
+    """Packed prompts captured once and replayed over other inputs, lengths and
+    slots: tiles, and long rows split in time."""
+    D, N, total = 64, 16, 3000
+    w = torch.randn(D, 4, device=cuda).to(BF)
+    s = _inputs(cuda, (1, total), D, N, 1, BF)
+    cu, ids = torch.tensor([0, 1400, 3000], device=cuda), torch.tensor([1, 2], dtype=torch.int32, device=cuda)
+    conv, ssm = torch.zeros(1, 4, 3, D, device=cuda, dtype=BF), torch.zeros(1, 4, D, N, device=cuda)
+
+    def call(v, c, h):
+        y = wk.short_conv_prefill_slots(v["x"], w, c, 0, ids, activation="silu", cu_seqlens=cu)
+        return _call(wk.selective_scan_prefill_slots, dict(v, x=y), h, 0, ids, cu_seqlens=cu)
+
+    call(s, conv, ssm)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = call(s, conv, ssm)
+    for seed, (offsets, slots) in enumerate([([0, 1400, 3000], [1, 2]), ([0, 3, 3000], [3, 1]), ([0, 2990, 2990], [2, 3])]):
+        fresh = _inputs(cuda, (1, total), D, N, 1, BF, seed=10 + seed)
+        for k in s:
+            s[k].copy_(fresh[k])
+        cu.copy_(torch.tensor(offsets, device=cuda))
+        ids.copy_(torch.tensor(slots, dtype=torch.int32, device=cuda))
+        conv.normal_()
+        ssm.normal_()
+        conv2, ssm2 = conv.clone(), ssm.clone()
+        graph.replay()
+        end = offsets[-1]
+        assert torch.equal(o[:, :end], call(fresh, conv2, ssm2)[:, :end])
+        assert torch.equal(conv, conv2) and torch.equal(ssm, ssm2)
+    ops.check_device_status(cuda)
+
+
+def test_conv_keeps_nan(cuda):
+    """A NaN reaches the W outputs whose window holds it and the state, in its channel alone."""
+    for T, D, W in ((5, 40, 4), (70, 40, 3), (70, 7, 4)):
+        x, w = torch.randn(2, T, D, device=cuda).to(BF), torch.randn(D, W, device=cuda).to(BF)
+        s0 = torch.randn(2, W - 1, D, device=cuda).to(BF)
+        o, st = wk.short_conv(x, w, activation="silu", initial_state=s0, output_final_state=True)
+        x[1, T - 2, 3] = s0[0, 0, 5] = float("nan")
+        o2, st2 = wk.short_conv(x, w, activation="silu", initial_state=s0, output_final_state=True)
+        mo, ms = torch.zeros_like(o, dtype=torch.bool), torch.zeros_like(st, dtype=torch.bool)
+        mo[1, T - 2:, 3] = mo[0, 0, 5] = ms[1, W - 3, 3] = True
+        assert torch.equal(o2.isnan(), mo) and torch.equal(st2.isnan(), ms)
+        assert torch.equal(o2[~mo], o[~mo]) and torch.equal(st2[~ms], st[~ms])
