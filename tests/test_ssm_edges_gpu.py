@@ -254,3 +254,34 @@ def test_conv_keeps_nan(cuda):
         mo[1, T - 2:, 3] = mo[0, 0, 5] = ms[1, W - 3, 3] = True
         assert torch.equal(o2.isnan(), mo) and torch.equal(st2.isnan(), ms)
         assert torch.equal(o2[~mo], o[~mo]) and torch.equal(st2[~ms], st[~ms])
+
+
+@pytest.mark.parametrize("n,T", [(256, 16), (200, 3), (64, 9)])
+def test_many_short_prompts_cost_what_their_tokens_do(cuda, n, T):
+    """Packed prompts of a few tokens each take about as long as the same
+    tokens in a batch: what a CTA does per sequence ahead of them is small."""
+    D, N = 2048, 16
+    a = _inputs(cuda, (1, n * T), D, N, 1, BF)
+    cu = torch.arange(0, n * T + 1, T, device=cuda)
+    h0 = torch.randn(n, D, N, device=cuda)
+    batch = {k: v.view(n, T, *v.shape[2:]) if k in ("x", "dt", "B", "C", "z") else v for k, v in a.items()}
+    calls = [lambda: _call(wk.selective_scan, a, initial_state=h0, output_final_state=True, cu_seqlens=cu),
+             lambda: _call(wk.selective_scan, batch, initial_state=h0, output_final_state=True)]
+    (o, ht), (o2, ht2) = (f() for f in calls)
+    times = []
+    for f in calls:
+        best = []
+        for _ in range(5):
+            b, e = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            b.record()
+            for _ in range(10):
+                f()
+            e.record()
+            e.synchronize()
+            best.append(b.elapsed_time(e))
+        times.append(min(best))
+    ro, tol, rh, htol = ssm_ref.scan(*[a[k][..., :64] if k in ("x", "dt") else a[k][:64] if k == "A" else a[k] for k in NAMES],
+                                     a["D"][:64], a["z"][..., :64], a["dt_bias"][:64], True, h0[:, :64], cu.tolist())
+    ssm_ref.check(o[..., :64], ro, tol, "o")
+    ssm_ref.check(ht[:, :64], rh, htol, "state")
+    assert times[0] < 5 * times[1], times

@@ -655,7 +655,11 @@ int launch_tiles(const ScanArgs& s, int parts, cudaStream_t st) {
             aligned_to(s.dt.p, ax) && aligned_to(s.o, ax) &&
             (!s.z.p || (even(s.z, K::VE) && aligned_to(s.z.p, ax)));
   q.vec_b = even(s.B, K::VB) && even(s.C, K::VB) && aligned_to(s.B.p, ab) && aligned_to(s.C.p, ab);
-  q.longest_first = s.seqs.cu && s.seqs.nseq > 1 && s.seqs.nseq <= 256;
+  // Every CTA compares all pairs of sequences for it, so it is for few and long
+  // ones: 16 unequal ones of 32768 x 2048 in all take 595 us against 837 without,
+  // 64 of them 579 against 605; but 64 of 2,048 tokens in all 85 against 66, 128
+  // of 32768 789 against 662, and 256 of 16 tokens each 2,281 against 157.
+  q.longest_first = s.seqs.cu && s.seqs.nseq > 1 && s.seqs.nseq <= 64 && s.seqs.T >= 4 * s.seqs.nseq * s.seqs.nseq;
   if (jobs * parts > INT32_MAX) return WKVM_ERR_SHAPE;
   constexpr auto kern = scan_tiles_kernel<T, N, NP, NS, NT, TT, CLUSTER>;
   constexpr int bytes = K::bytes(CLUSTER);
