@@ -349,7 +349,8 @@ int wkvm_short_conv_slots(
  * g = d / (D / G), N in {8, 16, 32, 64, 128}; A [D, N], D_skip [D] or NULL
  * and dt_bias [D] or NULL are fp32; states are fp32 [.., D, N]. `strides`
  * is a host array of ten: batch and token stride of x, dt, z, Bm, Cm.
- * h0 (optional) and ht (optional, may equal h0) are [B, D, N]. */
+ * h0 (optional) and ht (optional, may equal h0) are [B, D, N]. A and the
+ * states start on 16 bytes (WKVM_ERR_ALIGN). */
 int wkvm_selective_scan(
     const void* x, const void* dt, const float* A, const void* Bm, const void* Cm,
     const float* D_skip, const void* z, const float* dt_bias, void* o,

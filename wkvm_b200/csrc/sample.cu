@@ -28,10 +28,11 @@
 // larger set is narrowed by further histograms and drawn from by a pass over
 // the whole row. HBM is read once: later passes find the slice in shared
 // memory, or, in vocabularies too long for sixteen CTAs', in L2. At 256 rows of
-// 65,536 fp32 logits (10 us of HBM): 33 us greedy, 60 top-k 50, 70 without a
-// filter, 182 top-p 0.9 (thousands of tokens kept), which evaluates the weights
-// twice; the issue of some ninety instructions a logit bounds it, then the
-// latency of one row's phases (one row: 8, 14, 12 and 31 us).
+// 65,536 fp32 logits (10 us of HBM), on the device: 25 us greedy, 63 top-k and
+// top-p, 65 without a filter, 170 top-p 0.8 to 0.99 (thousands of tokens kept),
+// which evaluates the weights twice; 90 with a mix of settings. The issue of
+// some ninety instructions a logit bounds it, then the latency of one row's
+// phases (one row: 13 us top-k, 21 top-p).
 #include <cooperative_groups.h>
 #include <float.h>
 
@@ -931,9 +932,13 @@ extern "C" int wkvm_sample_tokens(const void* logits, int64_t row_stride, const 
   if (B == 0) return WKVM_OK;
   if (!logits || !u || !tokens || !logprobs) return WKVM_ERR_INVALID_ARG;
   // Slices of 16,384 fit shared memory and spread the rows that need several
-  // passes (256 mixed rows of 65,536: 98 us over four CTAs each, 158 whole, 117
-  // over eight). Few rows take more CTAs (one: 34 us over eight, 45 over four),
-  // sixteen only where all are resident at once.
+  // passes among those that do not: 256 rows of 65,536 with a mix of settings
+  // take 90 us over four CTAs each, 99 over two, 140 whole, 106 over eight. Rows
+  // that all need them gain nothing and pay the barriers: top-p for all 170 us
+  // over four, 158 over two, 154 whole; greedy 25, 24 and 20. Few rows take more
+  // CTAs (one under top-p: 21 us over sixteen, 24 over eight, 33 over four, 88
+  // whole; 32 mixed rows 33 over eight, 37 over sixteen), sixteen only where all
+  // are resident at once.
   int ctas = 1;
   while (ctas < 8 && (V > ctas * wkvm::kSmemSlice || ((int64_t)B * ctas <= 256 && V >= ctas * 2048))) ctas *= 2;
   if (ctas == 8 && (B <= 8 || V > 8 * wkvm::kSmemSlice) && V >= 16384) ctas = 16;

@@ -47,7 +47,10 @@ struct ScanArgs {
 constexpr int kRowThreads = 128;
 
 // A as a power of two's exponent; -FLT_MAX for -inf, so that a step of zero
-// keeps the state there too. NaN stays NaN (fmaxf would drop it).
+// keeps the state there too. NaN stays NaN (fmaxf would drop it). A decay is
+// 2^(delta (A log2 e)) with both products rounded: |delta A| 2^-23 of it beside
+// ex2's 2^-22. e^(delta A) would round one product only, for one more in the
+// inner loop of every state.
 __device__ __forceinline__ float scaled(float a) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a * kLog2e), "f"(-FLT_MAX));
@@ -168,11 +171,12 @@ __global__ void __launch_bounds__(kRowThreads, 8) scan_rows_kernel(ScanArgs p) {
 // ---------------------------------------------------------------------------
 // Tile kernel, for prompts. Its floor is T D N exponentials at 16 a clock and
 // SM (4.65e12 / s; 231 us for 32768 x 2048 x 16) rather than the 8 bytes of
-// activations per N of them (83 us). What bounds it is the issue of the other
-// instructions, some nine an exponential: at sixteen packed prompts of that
-// size it takes 594 us, the exponentials' pipe half busy, 0.6 instructions a
-// clock and scheduler from three warps (two channels to a register pair took
-// it from 880 us, straight-line tile phases and byte permutes to 594).
+// activations per N of them (83 us). Other instructions come to some nine an
+// exponential. Sixteen packed prompts of that size take 607 us (two channels to
+// a register pair took it from 880, straight-line tile phases and byte permutes
+// to this). Nothing is saturated there: the exponentials' pipe is half busy, and
+// a scheduler issues 0.6 instructions a clock from three warps, which wait for
+// their operands; the longest prompt's tail runs with fewer.
 //
 // One CTA walks one sequence for CB channels, TT tokens at a time. A thread
 // keeps NS states of CH channels; the L = N / NS threads of a channel leave
@@ -182,13 +186,16 @@ __global__ void __launch_bounds__(kRowThreads, 8) scan_rows_kernel(ScanArgs p) {
 // by the L threads: they read (delta, delta x) pairs. Shared memory gives
 // 128 bytes a clock however many lanes read the same word, so a thread's
 // share of B and C (kept in the inputs' dtype) is read once for its CH
-// channels. Inputs of the next tile are in registers while this one runs.
+// channels. The next tile's inputs are copied into shared memory while this one
+// runs, asynchronously where both sides are aligned.
 //
 // Few rows (a long prompt alone, few channels): the CTAs of a cluster split
 // the sequence's tiles between them. Each first runs its part from a zero
 // state for its final state and the sum of its steps (whose exponential is
 // the part's whole decay, A being constant), then takes the parts before it
 // from its peers' shared memory and runs its part again from its true start.
+// The sum of n steps is held in fp32: n 2^-24 of it at most, as much as the n
+// products of the tokens one by one lose.
 // ---------------------------------------------------------------------------
 // softplus() of two
 __device__ __forceinline__ f32x2 softplus2(f32x2 x) {
@@ -684,21 +691,28 @@ template <typename T, int N>
 int launch_scan_n(const ScanArgs& a, cudaStream_t st) {
   // a few tokens of every row: the state's traffic decides, so the row kernel
   if (!a.seqs.cu && a.seqs.T <= 8) {
-    // Four channels a thread once that still gives every SM a thousand threads
-    // (512 rows of 4096 x 16: 70 us, 62 % of the measured HBM rate; two 92 us;
-    // eight 113 us, as A and the states then take 162 registers).
+    // Four channels a thread once that still gives every SM a thousand threads.
+    // 512 rows of 4096 x 16, bf16, on the device: 60 us with four (4.7 TB/s, 72 %
+    // of the measured HBM rate), 75 with two, 112 with one, 86 with eight, which
+    // do not fit the 64 registers that eight blocks an SM leave. Few rows go the
+    // other way: one 2.9 us with one channel a thread, 3.5 with four; eight rows
+    // 3.7 and 4.1; sixteen 5.7 and 4.6.
     if ((int64_t)a.seqs.nseq * a.D * N / 16 >= 148 * 1024) return launch_rows<T, N, 4>(a, st);
     return launch_rows<T, N, 1>(a, st);
   }
   // Warps that four states (two channels) a thread give, of 592 schedulers.
-  // Few: sequences are split in time over clusters (one of 8192 x 4096: 469 us
-  // against 650 whole). A split pays twice for the exponentials, so it takes
-  // four parts at least and room for them. Sequences of unequal length, or not
-  // enough rows for two waves: fewer states a thread, so more warps (sixteen
-  // packed prompts of 32768 x 2048 in all: 630 us against 790). Else the wide
-  // form (16 equal ones of 2048: 500 us against 635). From 64 states on B and C
-  // outweigh a CTA's channels, so the fine form keeps four or eight states
-  // (three sequences of 666 x 1002, fp32: 110 us against 145 with two).
+  // Few: sequences are split in time over clusters (one of 8192 x 4096: 461 us
+  // in eight parts, 528 in four, 590 whole in the fine form, 892 in the wide). A
+  // split pays twice for the exponentials, so it takes four parts at least and
+  // room for them. It goes by the average length, as the host knows no other:
+  // one prompt of 8,192 beside 31 of four tokens stays whole (2048 channels: 594
+  // us, 315 in eight parts). Packed sequences, or not enough rows for two waves:
+  // the fine form, fewer states a thread and so more warps (sixteen unequal
+  // prompts of 32768 x 2048 in all: 607 us against 788 wide; sixteen equal ones,
+  // which the host cannot tell from them, 599 against 495). A batch of enough
+  // rows is of equal length: the wide form. From 64 states on B and C outweigh a
+  // CTA's channels, so the fine form keeps four or eight states (three sequences
+  // of 666 x 1002 x 64, fp32: 104 us; 103 in the wide form).
   constexpr int kWide = N == 128 ? 8 : 4;
   const int64_t warps = (int64_t)a.seqs.nseq * a.D * N / (kWide * 2 * 32);
   const int64_t tokens = a.seqs.cu ? a.seqs.T / a.seqs.nseq : a.seqs.T;

@@ -79,10 +79,12 @@ __device__ __forceinline__ float silu(float x) {
   return x * rcp(1.0f + ex2(-kLog2e * x));
 }
 
-// log(1 + e^x) to about 2^-21 relative, small values too: max(x, 0) +
-// log1p(e^-|x|). log1p(e) on [0, 1] is e times a polynomial of degree 8,
-// minimax in the relative error (Remez exchange, 3e-8; 2^-22.2 with fp32
-// rounding). The step scales every exponent of the scan, so it keeps fp32.
+// log(1 + e^x) = max(x, 0) + log1p(e^-|x|) in 32 bits, to 2^-20 (1 + |x| / 8)
+// relative: log1p(e) on [0, 1] is e times a polynomial of degree 8, minimax in
+// the relative error (Remez exchange, 3e-8; 2^-22.2 with fp32 rounding), ex2
+// holds 2^-22, and the rounded exponent |x| 2^-23.7. log1pf of expf would hold
+// some 2^-22 throughout; what is lost beside it is below the rounding of a
+// 16-bit dt, and for fp32 within a few steps of the result.
 __host__ __device__ constexpr float log1p_coeff(int i) {
   return i == 0 ? 0.99999994f : i == 1 ? -0.49999493f : i == 2 ? 0.33319098f : i == 3 ? -0.24842982f
        : i == 4 ? 0.19106007f : i == 5 ? -0.13663246f : i == 6 ? 0.078225955f : i == 7 ? -0.029505240f

@@ -11,8 +11,10 @@ request, and both states are families of a bank
 
 Activations are [B, T, D], or [1, total, D] with cu_seqlens; views whose last
 axis is contiguous (one half of a projection's output, a slice of it) are read
-where they are. Outputs are new contiguous tensors. The operators are
-forward only: inputs that ask for gradients are refused.
+where they are. Outputs are new contiguous tensors; tokens of a packed axis
+that no sequence covers are not written. Slot ids of one call differ, but for
+padding rows, which may share slot 0. The operators are forward only: inputs
+that ask for gradients are refused.
 """
 
 from __future__ import annotations
@@ -159,7 +161,8 @@ def short_conv(x, weight, bias=None, activation: str | None = None, initial_stat
     """Short causal convolution: o[t, d] = act(bias[d] + sum_j weight[d, j] x[t-W+1+j, d]).
 
     x [B, T, D] or packed [1, total, D] with ``cu_seqlens``; weight [D, W] (or
-    [D, 1, W]) with W in 2..4; activation None or "silu". ``initial_state``
+    [D, 1, W]) with W in 2..4; activation None or "silu". A weight, bias or
+    state of another dtype is rounded to x's; sums are fp32. ``initial_state``
     [N, W-1, D] in x's dtype holds the inputs before each sequence's first
     token, oldest first (None: zeros). Returns (o, final_state), the last W-1
     inputs of each sequence when ``output_final_state``, else None."""
@@ -288,8 +291,9 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus: bo
     x, dt, z [B, T, D] or packed [1, total, D] with ``cu_seqlens``; A [D, N];
     B, C [B, T, N] or [B, T, G, N], channel d in group g = d // (D // G);
     D, dt_bias [D]; z, D and dt_bias optional. N in 8, 16, 32, 64, 128.
-    States are fp32 [sequences, D, N]. Returns (o, final_state): o in x's
-    dtype, final_state fp32 when ``output_final_state``, else None."""
+    States are fp32 [sequences, D, N]; A and states start on 16 bytes.
+    Returns (o, final_state): o in x's dtype, final_state fp32 when
+    ``output_final_state``, else None."""
     a = _Scan(x, dt, A, B, C, D, z, dt_bias, initial_state, cu_seqlens)
     want = (a.nseq, a.d, a.n)
     if initial_state is not None and tuple(initial_state.shape) != want:

@@ -239,7 +239,7 @@ class SSMStateLayout:
 
 class SSMStateBank:
     """Slot-indexed states of selective state space layers, with the slot
-    operations of :class:`RWKV7StateBank`:
+    operations zero, fork, snapshot and restore:
 
       ssm  [L, S+1, D, N] fp32          (slot 0 = reserved padding row)
       conv [L, S+1, W-1, D] model dtype (the last W-1 inputs, oldest first)
