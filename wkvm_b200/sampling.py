@@ -44,10 +44,11 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     With w_i = exp((l_i - max l) / temperature): ``top_k`` keeps the k largest
     logits (0: all; a whole number, fractions in a tensor are rounded up);
     ``top_p`` keeps, of those in descending order, the shortest prefix that
-    holds at least that share of their mass (1: all); ``min_p`` keeps, of those, w_i >= min_p (0: all). The token is the first
-    kept id whose running mass, over ascending ids, exceeds u times the mass
-    kept (masses hold 2^-46 of the largest weight at 65,536 logits; less is
-    never drawn). Ties go to the lowest ids; temperature 0 is greedy. -inf (and NaN)
+    holds at least that share of their mass (1: all); ``min_p`` keeps, of
+    those, w_i >= min_p (0: all). The token is the first kept id whose running
+    mass, over ascending ids, exceeds u times the mass kept. Masses count in
+    units of 2^-46 at 65,536 logits; a weight of less than half a unit is never
+    drawn. Ties go to the lowest ids; temperature 0 is greedy. -inf (and NaN)
     logits are never chosen; a row of nothing else gives token -1 and
     log-probability -inf. The same inputs give the same tokens on every run,
     eagerly and in a captured graph. Forward only: inputs that ask for
